@@ -35,11 +35,12 @@ extern "C" {
 #define MME_ERR_HIP 2         /* HIP runtime error at launch               */
 #define MME_ERR_UNSUPPORTED 3 /* valid request this build does not handle  */
 
-#define MME_ABI_VERSION 9  /* 6: mme_gemm_res_stats row_part is [M][N / 64][2]; 7: mme_build_flags, mme_topk_rows_torch;
+#define MME_ABI_VERSION 10 /* 6: mme_gemm_res_stats row_part is [M][N / 64][2]; 7: mme_build_flags, mme_topk_rows_torch;
                               8: mme_recall_hits skip mask, mme_sim_scores, mme_tie_rows; per-call kernel
                                  forms (mme_*_form) replace the process-global *_variant switches, which
                                  remain in the development build only;
-                              9: mme_attention_qs (+ _form), Q pre-scaled */
+                              9: mme_attention_qs (+ _form), Q pre-scaled;
+                              10: mme_rope_axes, mme_attention_docs */
 
 /* mme_build_flags() bits */
 #define MME_BUILD_DEV 1 /* development / diagnostic kernel forms compiled in (libmme_dev.so) */
@@ -385,6 +386,38 @@ int mme_l2norm_masked(const void* x, int ldx, void* y, int ldy, int rows, int d,
  * out: bf16 [B*T, ld_out], head h at column h*256. */
 int mme_attention_mqa(const void* qkv, int ld_qkv, void* out, int ld_out, int B, int T, int Hq, int hd,
                       const int32_t* kstart, const int32_t* kend, float scale, void* stream);
+
+/* ------------------------------------- pages, images and texts packed together ----
+ * Rows of several documents lie one after the other; the two operators below need no padding. */
+
+/* Rotary positions with several axes (time, height, width, ...): pair i < pairs of each of the nheads heads
+ * (head h at column h*hd) turns by positions[axes[i] * ld_pos + row] * freqs[i] radians (double; the angle is
+ * reduced in 64 bits):  y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin, fp32, one rounding to bf16;
+ * (a, b) = (i, i + pairs), or (2i, 2i + 1) with `adjacent`. `inverse` turns back (the rotation's gradient).
+ * Elements 2*pairs .. hd of a head are copied. y may be x (ldy == ldx; those elements then stay untouched) or
+ * must not overlap it. axes[i] outside [0, naxes) is clamped. Any even / odd pairs, hd and leading dims; vectors
+ * of 16 or 8 bytes are used where 2*pairs, 2*hd, both leading dims and pointers (in bytes) allow it. */
+int mme_rope_axes(const void* x, long ldx, void* y, long ldy, int rows, int nheads, int hd, int pairs,
+                  const int32_t* positions, long ld_pos, int naxes, const double* freqs, const int32_t* axes,
+                  int adjacent, int inverse, void* stream);
+
+/* Attention over n packed documents. Document d has the query rows [q_offsets[d], q_offsets[d+1]) and the key rows
+ * [k_offsets[d], k_offsets[d+1]); the offsets (int32[n+1], not decreasing; clamped to the rows there are) may be the
+ * same array. Query i of a document stands at key position p = i + klen - qlen. It sees key j of its own document
+ * where  !causal,  or j <= p,  or j < prefix[d] (int32[n], nullable, with causal only). Its score is
+ *   x = scale q.k;  softcap > 0: x = softcap tanh(x / softcap);  slopes (fp32[Hq], nullable): x -= slopes[h] |p - j|
+ * and out = softmax(x) v over the keys it sees, 0 where it sees none. A key that a query does not see adds nothing
+ * to it, whatever k and v hold there. Rows of no document are left as they were, and so are a document's rows from
+ * max_rows on (max_rows: the most query rows a document has, or rows_q; small ones let long keys be split over the
+ * device and joined). q: bf16 [rows_q, ldq], head h at column h*hd; k, v: bf16 [rows_k, ld], key head h / (Hq/Hkv);
+ * out: bf16 [rows_q, ldo]. hd: multiples of 8 up to 128, of 16 up to 256. 16-byte aligned pointers, leading dims
+ * % 8 == 0. fp32 scores, softmax and sums; the weights are rounded to bf16 for the matrix instruction.
+ * workspace >= mme_attention_docs_workspace_bytes(...) (0: may be null). */
+size_t mme_attention_docs_workspace_bytes(int n, int rows_q, int rows_k, int Hq, int Hkv, int hd, int max_rows);
+int mme_attention_docs(const void* q, long ldq, const void* k, long ldk, const void* v, long ldv, void* out, long ldo,
+                       const int32_t* q_offsets, const int32_t* k_offsets, int n, int rows_q, int rows_k, int Hq,
+                       int Hkv, int hd, int max_rows, int causal, const int32_t* prefix, float softcap,
+                       const float* slopes, float scale, void* workspace, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

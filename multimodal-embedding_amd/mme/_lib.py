@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_float, c_int, c_int64, c_long, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # MME_DEV=1 loads the development build (every dev / diagnostic kernel form; `make dev`)
@@ -18,7 +18,7 @@ LIB_PATH = os.environ.get("MME_LIB", os.path.join(_HERE, "libmme_dev.so" if DEV 
 # MME_ACT_* / MME_PIX_* from include/mme.h
 ACT_NONE, ACT_GELU_TANH, ACT_QUICK_GELU, ACT_GELU_ERF, ACT_GEGLU_TANH = 0, 1, 2, 3, 4
 PIX_F32_NCHW, PIX_PATCHES = 0, 1
-ABI_VERSION = 9
+ABI_VERSION = 10
 BUILD_DEV = 1  # MME_BUILD_DEV
 
 # name -> (restype, argtypes)
@@ -68,6 +68,11 @@ SIGNATURES = {
     "mme_rope": (c_int, [_P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P]),
     "mme_gemma_embed": (c_int, [_P, c_int, c_int, _P, c_int, c_float, _P, c_int, c_int, _P, c_int, _P]),
     "mme_l2norm_masked": (c_int, [_P, c_int, _P, c_int, c_int, c_int, _P, _P]),
+    "mme_rope_axes": (c_int, [_P, c_long, _P, c_long, c_int, c_int, c_int, c_int, _P, c_long, c_int, _P, _P, c_int,
+                              c_int, _P]),
+    "mme_attention_docs_workspace_bytes": (c_size_t, [c_int] * 7),
+    "mme_attention_docs": (c_int, [_P, c_long, _P, c_long, _P, c_long, _P, c_long, _P, _P, c_int, c_int, c_int, c_int,
+                                   c_int, c_int, c_int, c_int, _P, c_float, _P, c_float, _P, c_size_t, _P]),
     "mme_attention_mqa": (c_int, [_P, c_int, _P, c_int, c_int, c_int, c_int, c_int, _P, _P, c_float, _P]),
 }
 # per-call kernel forms (ABI 8; mme.ops.kernel_forms): the entry point's arguments after an int form

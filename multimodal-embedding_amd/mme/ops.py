@@ -449,6 +449,128 @@ def attention_mqa(qkv: torch.Tensor, B: int, T: int, Hq: int, hd: int, *, kstart
     return out
 
 
+# ---------------------------------------------------------------- packed documents
+def _on_device_of(t: torch.Tensor, *ts: Optional[torch.Tensor]):
+    """A context in which t's device is the current one (so its stream is taken); all tensors lie there."""
+    for u in ts:
+        if u is not None and u.device != t.device:
+            raise ValueError(f"tensors on two devices: {t.device} and {u.device}")
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axes: torch.Tensor, nheads: int, *,
+              hd: Optional[int] = None, adjacent: bool = False, inverse: bool = False,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions with several axes (mme_rope_axes): pair i of heads [0, nheads) of each row turns by
+    positions[axes[i], row] * freqs[i].
+
+    x: bf16 [rows, >= nheads * hd] (hd defaults to x.shape[1] // nheads); positions: int32 [naxes, rows]; freqs:
+    float64 [pairs]; axes: int32 [pairs] (rope_axes_freqs makes both). The pair is elements (i, i + pairs) of a head,
+    or (2i, 2i + 1) with adjacent; elements from 2 * pairs on are copied. inverse turns back: the gradient with
+    respect to x is this of the gradient with respect to the result. out: None for a new tensor, x itself for in
+    place, or one that does not overlap x."""
+    _dev(x, positions, freqs, axes, out)
+    ldx = _rowmajor(x, "x")
+    rows, pairs = x.shape[0], freqs.numel()
+    hd = x.shape[1] // max(nheads, 1) if hd is None else hd
+    if x.dtype != BF16 or (out is not None and out.dtype != BF16):
+        raise ValueError("rope_axes: x and out must be bf16")
+    if nheads < 1 or pairs < 1 or 2 * pairs > hd or nheads * hd > x.shape[1]:
+        raise ValueError(f"rope_axes: {nheads} heads of {hd} with {pairs} pairs do not fit rows of {x.shape[1]}")
+    if positions.dtype != torch.int32 or positions.dim() != 2 or positions.shape[1] != rows or positions.shape[0] < 1 \
+            or (rows > 1 and positions.stride(1) != 1):
+        raise ValueError(f"rope_axes: positions must be int32 [axes, {rows}] with contiguous rows")
+    if freqs.dtype != torch.float64 or axes.dtype != torch.int32 or axes.numel() != pairs or freqs.dim() != 1 \
+            or not (freqs.is_contiguous() and axes.is_contiguous()):
+        raise ValueError("rope_axes: freqs must be contiguous float64 [pairs] and axes int32 [pairs]")
+    with _on_device_of(x, positions, freqs, axes, out):
+        if out is None:
+            out = torch.empty(rows, nheads * hd, dtype=BF16, device=x.device)
+        elif out.dim() != 2 or out.shape[0] != rows or out.shape[1] < nheads * hd:
+            raise ValueError(f"rope_axes: out must be [{rows}, >= {nheads * hd}]")
+        ev = KernelTimer.begin()
+        call("mme_rope_axes", x.data_ptr(), ldx, out.data_ptr(), _rowmajor(out, "out"), rows, nheads, hd, pairs,
+             positions.data_ptr(), max(positions.stride(0), rows), positions.shape[0], freqs.data_ptr(),
+             axes.data_ptr(), int(adjacent), int(inverse), _stream())
+        KernelTimer.end(ev, "rope_axes", 0.0, 4.0 * rows * nheads * hd)
+    return out
+
+
+def rope_axes_freqs(sections: Sequence[int], theta: float, *, in_turns: bool = False, per_axis: bool = False,
+                    device="cuda"):
+    """(freqs float64 [pairs], axes int32 [pairs]) for rope_axes: sections[a] pairs turn with axis a, in blocks or
+    with the axes in turn (a, b, c, a, b, c, ... while each has pairs left). Pair i has the frequency
+    theta^(-i / pairs), or, per_axis, its axis's j-th pair has theta^(-j / sections[a])."""
+    if not sections or min(sections) < 0 or sum(sections) < 1 or not theta > 0:
+        raise ValueError(f"rope_axes_freqs: sections {tuple(sections)}, theta {theta}")
+    if in_turns:
+        order = [a for j in range(max(sections)) for a, s in enumerate(sections) if j < s]
+    else:
+        order = [a for a, s in enumerate(sections) for _ in range(s)]
+    seen, freqs = [0] * len(sections), []
+    for i, a in enumerate(order):
+        freqs.append(theta ** -(seen[a] / sections[a] if per_axis else i / len(order)))
+        seen[a] += 1
+    return (torch.tensor(freqs, dtype=torch.float64, device=device),
+            torch.tensor(order, dtype=torch.int32, device=device))
+
+
+def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, heads: int,
+                   kv_heads: int, *, key_offsets: Optional[torch.Tensor] = None, max_rows: Optional[int] = None,
+                   causal: bool = False, prefix: Optional[torch.Tensor] = None, softcap: float = 0.0,
+                   slopes: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(score(q, k)) v within each of the documents packed in the rows (mme_attention_docs).
+
+    q: bf16 [rows, heads * hd]; k, v: bf16 [key rows, kv_heads * hd] (views of packed q | k | v rows will do); each
+    key head serves heads / kv_heads query heads. offsets: int32 [n + 1], where each document's query rows begin;
+    key_offsets: the same for the keys (default: offsets). Query i of a document stands at key position
+    i + klen - qlen. causal: it sees keys up to its own position, and with prefix (int32 [n]) also the document's
+    first prefix[d] keys. softcap > 0: scores become softcap * tanh(score / softcap). slopes (fp32 [heads]): scores
+    lose slopes[h] * distance. A query that sees no key gets zeros; keys that it does not see add nothing, whatever
+    they hold. max_rows: no document has more query rows than this; give it where rows are few and keys many (one
+    query a document: max_rows=1), so that the keys are split over the device. Rows of no document, and a document's
+    rows from max_rows on, are left as they were (not set in a new out)."""
+    key_offsets = offsets if key_offsets is None else key_offsets
+    _dev(q, k, v, offsets, key_offsets, prefix, slopes, out)
+    ldq, ldk, ldv = _rowmajor(q, "q"), _rowmajor(k, "k"), _rowmajor(v, "v")
+    if heads < 1 or kv_heads < 1 or heads % kv_heads or q.shape[1] % heads:
+        raise ValueError(f"attention_docs: {heads} heads over {kv_heads} key heads in rows of {q.shape[1]}")
+    hd, rows, keys, n = q.shape[1] // heads, q.shape[0], k.shape[0], offsets.numel() - 1
+    if any(t.dtype != BF16 for t in (q, k, v)) or (out is not None and out.dtype != BF16):
+        raise ValueError("attention_docs: q, k, v and out must be bf16")
+    if k.shape != v.shape or k.shape[1] != kv_heads * hd:
+        raise ValueError(f"attention_docs: k {tuple(k.shape)} and v {tuple(v.shape)} must be [keys, {kv_heads * hd}]")
+    if n < 0 or key_offsets.numel() != n + 1 or any(
+            t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() for t in (offsets, key_offsets)):
+        raise ValueError("attention_docs: offsets and key_offsets must be contiguous int32 [documents + 1]")
+    if prefix is not None and (prefix.dtype != torch.int32 or prefix.numel() != n or not prefix.is_contiguous()):
+        raise ValueError("attention_docs: prefix must be contiguous int32 [documents]")
+    if prefix is not None and not causal:
+        raise ValueError("attention_docs: a prefix goes with the causal mask")
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.numel() != heads or not slopes.is_contiguous()):
+        raise ValueError("attention_docs: slopes must be contiguous fp32 [heads]")
+    if max_rows is not None and max_rows < 0:
+        raise ValueError("attention_docs: max_rows must not be negative")
+    max_rows = rows if max_rows is None else min(int(max_rows), rows)
+    scale = hd ** -0.5 if scale is None else scale
+    with _on_device_of(q, k, v, offsets, key_offsets, prefix, slopes, out):
+        if out is None:
+            out = torch.empty(rows, heads * hd, dtype=BF16, device=q.device)
+        elif out.dim() != 2 or out.shape[0] != rows or out.shape[1] < heads * hd:
+            raise ValueError(f"attention_docs: out must be [{rows}, >= {heads * hd}]")
+        wsb = query("mme_attention_docs_workspace_bytes", n, rows, keys, heads, kv_heads, hd, max_rows)
+        # a workspace of the call's own: calls on two streams, or in two captured graphs, share none
+        ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
+        ev = KernelTimer.begin()
+        call("mme_attention_docs", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(),
+             _rowmajor(out, "out"), offsets.data_ptr(), key_offsets.data_ptr(), n, rows, keys, heads, kv_heads, hd,
+             max_rows, int(causal), _ptr(prefix), float(softcap), _ptr(slopes), float(scale), _ptr(ws), wsb, _stream())
+        # which pairs are visible is on the device: the bytes alone are known here
+        KernelTimer.end(ev, "attention_docs", 0.0, 4.0 * rows * heads * hd + 4.0 * keys * kv_heads * hd)
+    return out
+
+
 # ---------------------------------------------------------------- embeddings
 def token_embed(ids: torch.Tensor, tok: torch.Tensor, pos: torch.Tensor, out: Optional[torch.Tensor] = None):
     _dev(ids, tok, pos, out)

@@ -1,0 +1,439 @@
+"""Rotary positions with several axes and attention over packed documents, against the 64-bit oracle."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import docs as oracle
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+HALF = 2.0 ** -8   # half a bf16 step, relative
+
+
+def randn(g, *shape, scale=1.0):
+    return (torch.randn(*shape, generator=g) * scale).to(BF16)
+
+
+def gen(*seed):
+    return torch.Generator().manual_seed(hash(seed) % (1 << 31) if len(seed) > 1 else seed[0])
+
+
+# ------------------------------------------------------------------ rope_axes
+def check_rope(y, x, pos, freqs, axes, nheads, hd, **kw):
+    want, size = oracle.rope_axes(x.double().numpy(), pos.numpy(), freqs.numpy(), axes.numpy(), nheads, hd, **kw)
+    got = y.double().cpu().numpy()[:, :nheads * hd]
+    # the rounding of the result, and of the sine and cosine: the fraction of a turn in fp32 (2^-25 turns = 2^-22.3)
+    # and the sine unit's own error, taken at 2^-19 in all, and three fp32 roundings of the products
+    tol = HALF * np.abs(want) + (2.0 ** -19 + 3 * 2.0 ** -24) * size
+    assert (np.abs(got - want) <= tol).all(), np.max(np.abs(got - want) - tol)
+
+
+ROPE = [
+    # rows, heads, hd, sections, theta, in_turns, per_axis, adjacent, far
+    (1, 1, 64, (32,), 1e4, False, False, False, 1),
+    (21, 9, 256, (32, 48, 48), 1e4, False, False, False, 1000),
+    (130, 5, 72, (18, 18), 1e4, False, True, False, 64),          # 8-byte vectors
+    (67, 3, 80, (10, 10, 10, 10), 1e2, True, False, True, 5000),
+    (33, 24, 64, (8, 8, 8), 1e6, True, False, True, 1000000),      # three quarters of a head
+    (40, 2, 72, (9, 8), 1e4, False, True, False, 300),             # single elements
+    (40, 2, 30, (5, 4), 1e4, True, True, True, 300),
+    (9, 3, 2, (1,), 1e4, False, False, False, 100),
+    (300, 1, 128, (64,), 1e4, False, False, False, 2147483000),    # the far end of int32
+    (257, 40, 64, (0, 32), 1e4, False, False, True, 100),          # an axis with no pairs; several heads a thread
+    (3000, 33, 64, (16, 8), 1e4, False, False, False, 100),
+]
+
+
+@pytest.mark.parametrize("case", ROPE, ids=lambda c: "x".join(map(str, c[:3])))
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rope_axes(cuda, case, inverse):
+    from mme import ops
+    rows, heads, hd, sections, theta, turns, per_axis, adjacent, far = case
+    g = gen(rows * 7 + hd)
+    x = randn(g, rows, heads * hd)
+    pos = torch.randint(-far // 2, far, (len(sections), rows), generator=g, dtype=torch.int64).to(torch.int32)
+    freqs, axes = ops.rope_axes_freqs(sections, theta, in_turns=turns, per_axis=per_axis, device=cuda)
+    args = (pos.to(cuda), freqs, axes, heads)
+    y = ops.rope_axes(x.to(cuda), *args, adjacent=adjacent, inverse=inverse)
+    few = slice(0, 200)
+    check_rope(y[few], x[few], pos[:, few], freqs.cpu(), axes.cpu(), heads, hd, adjacent=adjacent, inverse=inverse)
+    z = x.to(cuda)
+    assert ops.rope_axes(z, *args, adjacent=adjacent, inverse=inverse, out=z) is z
+    assert torch.equal(z, y)
+
+
+def test_rope_axes_strides_and_what_it_leaves(cuda):
+    """Views of packed q | k | v rows: the first heads turn, the rest and the rows' other columns stay."""
+    from mme import ops
+    g = gen(3)
+    x = randn(g, 50, 9 * 72 + 16).to(cuda)
+    pos = torch.randint(0, 99, (2, 64), generator=g).to(torch.int32).to(cuda)[:, :50]
+    freqs, axes = ops.rope_axes_freqs((18, 18), 1e4, per_axis=True, device=cuda)
+    keep = x.clone()
+    out = torch.full((50, 10 * 72), 7.0, dtype=BF16, device=cuda)
+    ops.rope_axes(x, pos, freqs, axes, 5, hd=72, out=out)
+    assert torch.equal(x, keep) and (out[:, 5 * 72:] == 7).all()
+    check_rope(out, x.cpu(), pos.cpu(), freqs.cpu(), axes.cpu(), 5, 72)
+    ops.rope_axes(x, pos, freqs, axes, 5, hd=72, out=x)
+    assert torch.equal(x[:, :360], out[:, :360]) and torch.equal(x[:, 360:], keep[:, 360:])
+    # odd leading dims and a base off 16 bytes
+    odd = randn(g, 20, 2 * 64 + 3).to(cuda)[:, 1:]
+    f1, a1 = ops.rope_axes_freqs((32,), 1e4, device=cuda)
+    p1 = torch.arange(20, dtype=torch.int32, device=cuda)[None]
+    check_rope(ops.rope_axes(odd, p1, f1, a1, 2, hd=64), odd.cpu(), p1.cpu(), f1.cpu(), a1.cpu(), 2, 64)
+    # axes outside the positions are clamped, no rows are no work
+    a2 = torch.full_like(a1, 5)
+    assert torch.equal(ops.rope_axes(odd, p1, f1, a2, 2, hd=64), ops.rope_axes(odd, p1, f1, a1, 2, hd=64))
+    assert ops.rope_axes(odd[:0], p1[:, :0], f1, a1, 2, hd=64).shape == (0, 128)
+
+
+def test_rope_axes_gradient_is_the_inverse(cuda):
+    """<g, d rope(x)/dx . u> by a difference along u (the map is linear) against <rope_inverse(g), u>."""
+    from mme import ops
+    g = gen(5)
+    x, u, w = (randn(g, 64, 4 * 64).to(cuda) for _ in range(3))
+    pos = torch.randint(0, 500, (3, 64), generator=g).to(torch.int32).to(cuda)
+    freqs, axes = ops.rope_axes_freqs((10, 11, 11), 1e4, device=cuda)
+    along = ops.rope_axes(u, pos, freqs, axes, 4).double()
+    back = ops.rope_axes(w, pos, freqs, axes, 4, inverse=True).double()
+    lhs, rhs = (w.double() * along).sum(), (back * u.double()).sum()
+    # each of the 2 x 16384 products is off by half a bf16 step at most
+    tol = HALF * ((w.double() * along).abs().sum() + (back * u.double()).abs().sum())
+    assert (lhs - rhs).abs() <= tol
+
+
+def test_rope_axes_refusals(cuda):
+    from mme import ops
+    x = torch.zeros(4, 128, dtype=BF16, device=cuda)
+    pos = torch.zeros(1, 4, dtype=torch.int32, device=cuda)
+    f, a = ops.rope_axes_freqs((32,), 1e4, device=cuda)
+    ops.rope_axes(x, pos, f, a, 2)
+    for bad in (lambda: ops.rope_axes(x.float(), pos, f, a, 2), lambda: ops.rope_axes(x, pos.long(), f, a, 2),
+                lambda: ops.rope_axes(x, pos[:, :3], f, a, 2), lambda: ops.rope_axes(x, pos, f.float(), a, 2),
+                lambda: ops.rope_axes(x, pos, f, a[:5], 2), lambda: ops.rope_axes(x, pos, f, a, 3),
+                lambda: ops.rope_axes(x, pos, f, a, 0), lambda: ops.rope_axes(x, pos, f, a, 2, hd=65),
+                lambda: ops.rope_axes(x, pos, f, a, 2, hd=60), lambda: ops.rope_axes(x.t(), pos, f, a, 2),
+                lambda: ops.rope_axes(x, pos, f, a, 2, out=x[:, :100]), lambda: ops.rope_axes(x.cpu(), pos, f, a, 2),
+                lambda: ops.rope_axes_freqs((), 1e4), lambda: ops.rope_axes_freqs((-1, 2), 1e4),
+                lambda: ops.rope_axes_freqs((0, 0), 1e4), lambda: ops.rope_axes_freqs((4,), 0.0)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+# ------------------------------------------------------------------ attention_docs
+def cuts(lens, first=0):
+    return torch.tensor(np.concatenate([[0], np.cumsum(lens)]) + first, dtype=torch.int32)
+
+
+def check_docs(got, q, k, v, offsets, heads, kv_heads, **kw):
+    f = lambda t: None if t is None else t.double().cpu().numpy() if t.is_floating_point() else t.cpu().numpy()  # noqa: E731
+    kw = {n: f(t) if isinstance(t, torch.Tensor) else t for n, t in kw.items()}
+    want, spread, reach = oracle.attention_docs(f(q), f(k), f(v), f(offsets), heads, kv_heads, **kw)
+    got = got.double().cpu().numpy()
+    hd = q.shape[1] // heads
+    # weights: half a bf16 step each before the products, and again where their sum is of the rounded ones; the result:
+    # half a step. Scores: hd fp32 additions of terms whose sizes sum to `reach`, the scaling, bias and maximum (4
+    # roundings), the tanh (3 roundings of the cap), exp2 and sums of fp32 (2^-20 takes 16 roundings).
+    delta = (hd + 4) * 2.0 ** -24 * np.repeat(reach, hd, 1) + 3 * kw.get("softcap", 0.0) * 2.0 ** -23 + 2.0 ** -20
+    tol = HALF * (spread + 2 * np.abs(want)) + 2 * (spread + np.abs(want)) * delta
+    tol += want.shape[0] * 2.0 ** -24 * spread
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (np.argwhere(bad)[:5], got[bad][:5], want[bad][:5], tol[bad][:5])
+
+
+def make(g, rows, keys, heads, kv_heads, hd, cuda, qscale=2.0, pad=0):
+    q = randn(g, rows, heads * hd + pad, scale=qscale).to(cuda)[:, :heads * hd]
+    kv = randn(g, keys, 2 * kv_heads * hd + pad).to(cuda)
+    return q, kv[:, :kv_heads * hd], kv[:, kv_heads * hd:2 * kv_heads * hd]
+
+
+HEADS = [(1, 1, 64), (4, 4, 72), (8, 1, 256), (6, 2, 80), (4, 1, 128), (3, 3, 8), (2, 1, 40), (5, 5, 96), (7, 1, 120),
+         (2, 2, 144), (3, 1, 208)]
+LENS = [(1,), (33, 1, 64, 0, 65, 128), (5, 77, 12, 31, 32), (0, 0, 300), (129, 2)]
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", HEADS)
+@pytest.mark.parametrize("lens", LENS, ids=lambda t: "_".join(map(str, t)))
+@pytest.mark.parametrize("mask", ["all", "causal", "prefix"])
+def test_docs_masks_and_widths(cuda, heads, kv_heads, hd, lens, mask):
+    from mme import ops
+    g = gen(hd * 31 + sum(lens))
+    q, k, v = make(g, sum(lens), sum(lens), heads, kv_heads, hd, cuda)
+    off = cuts(lens).to(cuda)
+    kw = dict(causal=mask != "all")
+    if mask == "prefix":
+        kw["prefix"] = torch.tensor([(3 * n) // 4 if i % 3 else n + 5 if i else 0 for i, n in enumerate(lens)],
+                                    dtype=torch.int32, device=cuda)
+    got = ops.attention_docs(q, k, v, off, heads, kv_heads, **kw)
+    check_docs(got, q, k, v, off, heads, kv_heads, **kw)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", [(4, 4, 64), (8, 1, 256), (4, 2, 128), (3, 3, 72)])
+@pytest.mark.parametrize("cap,bias,scale", [(50.0, False, None), (5.0, False, 1.0), (0.0, True, None), (30.0, True, 0.3),
+                                            (0.0, False, 4.0)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_docs_scores(cuda, heads, kv_heads, hd, cap, bias, scale, causal):
+    from mme import ops
+    lens = (70, 3, 200, 64)
+    g = gen(hd + int(cap))
+    q, k, v = make(g, sum(lens), sum(lens), heads, kv_heads, hd, cuda)
+    off = cuts(lens).to(cuda)
+    kw = dict(causal=causal, softcap=cap, scale=scale,
+              slopes=(2.0 ** -torch.arange(1, heads + 1).float()).to(cuda) if bias else None)
+    check_docs(ops.attention_docs(q, k, v, off, heads, kv_heads, **kw), q, k, v, off, heads, kv_heads, **kw)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", [(8, 1, 256), (4, 4, 72), (8, 2, 128), (1, 1, 64)])
+@pytest.mark.parametrize("klens", [(1030,), (5000, 1, 0, 777, 64, 2050), (129,) * 9])
+@pytest.mark.parametrize("qlen", [1, 3])
+@pytest.mark.parametrize("full", [False, True])
+def test_docs_few_queries(cuda, heads, kv_heads, hd, klens, qlen, full):
+    """Few rows against many keys, split and joined: documents without keys, fewer keys than queries, chunks that
+    causal rows do not reach."""
+    from mme import ops
+    g = gen(hd + qlen + len(klens))
+    n = len(klens)
+    qlens = [qlen if i != 2 else 0 if qlen > 1 else 1 for i in range(n)]
+    q, k, v = make(g, sum(qlens), sum(klens), heads, kv_heads, hd, cuda)
+    off, koff = cuts(qlens).to(cuda), cuts(klens).to(cuda)
+    kw = dict(key_offsets=koff, max_rows=qlen)
+    if full:
+        kw.update(causal=True, softcap=30.0, slopes=(2.0 ** -torch.arange(4, heads + 4).float()).to(cuda),
+                  prefix=torch.tensor([i * 3 for i in range(n)], dtype=torch.int32, device=cuda))
+    got = ops.attention_docs(q, k, v, off, heads, kv_heads, **kw)
+    check_docs(got, q, k, v, off, heads, kv_heads, **kw)
+    # without the promise the rows take the other way, to the same values
+    kw.pop("max_rows")
+    check_docs(ops.attention_docs(q, k, v, off, heads, kv_heads, **kw), q, k, v, off, heads, kv_heads, **kw)
+
+
+def test_docs_rows_that_see_nothing_are_zero(cuda):
+    from mme import ops
+    g = gen(11)
+    q, k, v = make(g, 90, 40, 2, 1, 64, cuda)
+    off, koff = cuts((50, 40)).to(cuda), cuts((40, 0)).to(cuda)
+    for max_rows in (None, 50):
+        got = ops.attention_docs(q, k, v, off, 2, 1, key_offsets=koff, causal=True, max_rows=max_rows)
+        check_docs(got, q, k, v, off, 2, 1, key_offsets=koff, causal=True)
+        assert (got[:10] == 0).all() and (got[50:] == 0).all()
+    none = ops.attention_docs(q, k[:0], v[:0], off, 2, 1, key_offsets=torch.zeros_like(off))
+    assert (none == 0).all()
+
+
+@pytest.mark.parametrize("split", [False, True])
+def test_docs_rows_left_alone(cuda, split):
+    """Rows before the first document, behind the last and past max_rows keep what they held; out may be wider."""
+    from mme import ops
+    g = gen(12)
+    q, k, v = make(g, 30, 4000, 4, 2, 64, cuda, pad=24)
+    off = torch.tensor([4, 6, 6, 11], dtype=torch.int32, device=cuda)
+    koff = torch.tensor([100, 1500, 1600, 3900], dtype=torch.int32, device=cuda)
+    big = torch.full((30, 4 * 64 + 8), 7.0, dtype=BF16, device=cuda)
+    kw = dict(key_offsets=koff, max_rows=3, out=big[:, :256])
+    assert ops.attention_docs(q, k, v, off, 4, 2, causal=not split, **kw).data_ptr() == big.data_ptr()
+    before = torch.full((30, 256), 7.0)
+    check_docs(big[:, :256], q, k, v, off, 4, 2, key_offsets=koff, max_rows=3, out=before, causal=not split)
+    assert (big[:4] == 7).all() and (big[9:] == 7).all() and (big[:, 256:] == 7).all()
+
+
+@pytest.mark.parametrize("hd", [64, 72, 128, 256])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_docs_what_masked_keys_hold_does_not_matter(cuda, hd, value):
+    """Infinities and NaN in k and v: beside the documents, in another document, and at keys that some rows of a
+    tile see and others do not."""
+    from mme import ops
+    g = gen(13)
+    lens = (70, 90, 33)
+    q, k, v = make(g, 200, 200, 2, 1, hd, cuda)
+    off = cuts(lens, first=2).to(cuda)
+    for t in (k, v):
+        t[:2] = value
+        t[195:] = value
+        t[2 + 70 + 41] = value      # key 41 of the second document: rows from 41 on see it when causal
+    bad = np.zeros(200, bool)
+    bad[2 + 70 + 41:2 + 160] = True
+    got = ops.attention_docs(q, k, v, off, 2, 1, causal=True)
+    clean_k, clean_v = k.clone(), v.clone()
+    for t in (clean_k, clean_v):
+        t[~torch.isfinite(t)] = 0
+    clean = ops.attention_docs(q, clean_k, clean_v, off, 2, 1, causal=True)
+    inside = np.zeros(200, bool)
+    inside[2:195] = True
+    good = torch.from_numpy(inside & ~bad).to(cuda)
+    assert torch.isfinite(got[good].float()).all()
+    # the odd path adds key by key: the same fp32 sums in another order
+    assert torch.allclose(got[good].float(), clean[good].float(), rtol=2 * HALF, atol=2.0 ** -16)
+    if value != value:
+        assert torch.isnan(got[2 + 70 + 41:2 + 160].float()).all()
+
+
+def test_docs_values_that_reach_far(cuda):
+    """Scores of +-1e30, all alike, and a maximum that grows in every tile."""
+    from mme import ops
+    g = gen(14)
+    q, k, v = make(g, 256, 256, 1, 1, 64, cuda)
+    off = cuts((256,)).to(cuda)
+    for f in (1e15, 0.0):
+        got = ops.attention_docs((q.float() * f).to(BF16), (k.float() * max(f, 1)).to(BF16), v, off, 1, 1)
+        want, _, _ = oracle.attention_docs((q.float() * f).to(BF16).double().cpu().numpy(),
+                                           (k.float() * max(f, 1)).to(BF16).double().cpu().numpy(),
+                                           v.double().cpu().numpy(), off.cpu().numpy(), 1, 1)
+        # at 1e30 a row is its largest key's value (no two keys of these inputs tie)
+        assert np.allclose(got.double().cpu().numpy(), want, rtol=4 * HALF, atol=2 * HALF)
+    up = (torch.arange(256).float()[:, None] / 8).expand(256, 64).to(BF16).to(cuda)
+    ones = torch.ones(256, 64, dtype=BF16, device=cuda)
+    check_docs(ops.attention_docs(ones, up, v, off, 1, 1), ones, up, v, off, 1, 1)
+
+
+def test_docs_many_documents(cuda):
+    """5 000 documents, empty ones among them: the search for a slot's document goes several steps."""
+    from mme import ops
+    r = np.random.RandomState(1)
+    lens = r.randint(0, 4, 5000)
+    g = gen(15)
+    q, k, v = make(g, int(lens.sum()), int(lens.sum()), 2, 1, 64, cuda)
+    off = cuts(lens).to(cuda)
+    check_docs(ops.attention_docs(q, k, v, off, 2, 1, causal=True), q, k, v, off, 2, 1, causal=True)
+    klens = r.randint(200, 500, 300)
+    q, k, v = make(g, 300, int(klens.sum()), 2, 2, 64, cuda)
+    off, koff = cuts([1] * 300).to(cuda), cuts(klens).to(cuda)
+    got = ops.attention_docs(q, k, v, off, 2, 2, key_offsets=koff, max_rows=1)
+    check_docs(got, q, k, v, off, 2, 2, key_offsets=koff)
+
+
+def test_docs_far_into_a_long_cache(cuda):
+    """Keys whose elements lie past 2^31 and 2^32 from the cache's begin."""
+    from mme import ops
+    rows, ld = 540000, 8192   # 4.4e9 elements, 8.8 GB
+    cache = torch.zeros(rows, ld, dtype=BF16, device=cuda)
+    koff = torch.tensor([263000, 264000, 539200, 540000], dtype=torch.int32, device=cuda)
+    g = gen(16)
+    for a, b in ((263000, 264000), (539200, 540000)):
+        cache[a:b, :256] = randn(g, b - a, 256).to(cuda)
+    off = torch.tensor([0, 2, 2, 5], dtype=torch.int32, device=cuda)
+    q = randn(g, 5, 4 * 64).to(cuda)
+    k, v = cache[:, :128], cache[:, 128:256]
+    got = ops.attention_docs(q, k, v, off, 4, 2, key_offsets=koff, max_rows=3)
+    wide = ops.attention_docs(q, k, v, off, 4, 2, key_offsets=koff)
+    part = torch.cat([cache[263000:264000, :256], cache[539200:540000, :256]])
+    less = torch.tensor([0, 1000, 1000, 1800], dtype=torch.int32)
+    for out in (got, wide):
+        check_docs(out, q, part[:, :128], part[:, 128:], off, 4, 2, key_offsets=less)
+
+
+def test_docs_wrong_offsets_stay_inside(cuda):
+    """Offsets past the rows, negative or falling are clamped: rows come out wrong, nothing else is touched."""
+    from mme import ops
+    g = gen(17)
+    q, k, v = make(g, 64, 600, 2, 1, 64, cuda)
+    out = torch.full((66, 128), 7.0, dtype=BF16, device=cuda)
+    for off, koff in (([-5, 20, 1000], [0, 700, 2000000000]), ([40, 10, 64], [600, 3, 100]),
+                      ([0, 64, 64], [-2147483648, 2147483647, 5])):
+        for max_rows in (None, 4):
+            ops.attention_docs(q, k, v, torch.tensor(off, dtype=torch.int32, device=cuda), 2, 1, max_rows=max_rows,
+                               key_offsets=torch.tensor(koff, dtype=torch.int32, device=cuda), out=out[1:65])
+    torch.cuda.synchronize()
+    assert (out[0] == 7).all() and (out[65] == 7).all()
+
+
+def test_docs_refusals(cuda):
+    from mme import _lib, ops
+    q = torch.zeros(10, 4 * 64, dtype=BF16, device=cuda)
+    k = torch.zeros(10, 2 * 64, dtype=BF16, device=cuda)
+    off = torch.tensor([0, 10], dtype=torch.int32, device=cuda)
+    pre = torch.zeros(1, dtype=torch.int32, device=cuda)
+    slopes = torch.zeros(4, device=cuda)
+    ok = ops.attention_docs(q, k, k, off, 4, 2, causal=True, prefix=pre, slopes=slopes, softcap=1.0)
+    assert (ok == 0).all()
+    assert ops.attention_docs(q, k, k, off[:1], 4, 2).shape == q.shape       # no document
+    assert ops.attention_docs(q[:0], k, k, off * 0, 4, 2).shape == (0, 256)
+    f = ops.attention_docs
+    for bad in (lambda: f(q.float(), k, k, off, 4, 2), lambda: f(q, k, k.half(), off, 4, 2),
+                lambda: f(q, k, k[:5], off, 4, 2), lambda: f(q, k, k, off, 4, 3), lambda: f(q, k, k, off, 3, 1),
+                lambda: f(q, k, k, off.long(), 4, 2), lambda: f(q, k, k, off[:0], 4, 2),
+                lambda: f(q, k, k, off, 4, 2, key_offsets=off[:1]), lambda: f(q, k, k, off, 4, 2, prefix=pre),
+                lambda: f(q, k, k, off, 4, 2, causal=True, prefix=pre.long()),
+                lambda: f(q, k, k, off, 4, 2, causal=True, prefix=off), lambda: f(q, k, k, off, 4, 2, slopes=slopes[:2]),
+                lambda: f(q, k, k, off, 4, 2, slopes=slopes.double()), lambda: f(q, k, k, off, 4, 2, max_rows=-1),
+                lambda: f(q.cpu(), k, k, off, 4, 2), lambda: f(q, k.t(), k, off, 4, 2),
+                lambda: f(q, k, k, off, 4, 2, out=q[:5]), lambda: f(q, k, k, off, 4, 2, out=q[:, :128]),
+                lambda: f(q, k, k, off, 4, 2, out=q.float())):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: f(q, k, k, off, 4, 2, scale=0.0), lambda: f(q, k, k, off, 4, 2, scale=float("inf")),
+                lambda: f(q, k, k, off, 4, 2, scale=float("nan")), lambda: f(q, k, k, off, 4, 2, softcap=-1.0),
+                lambda: f(q, k, k, off, 4, 2, softcap=float("nan")),
+                lambda: f(q[:, :4 * 12], k[:, :2 * 12], k[:, :2 * 12], off, 4, 2),           # head dim 12
+                lambda: f(q[:, 4:4 + 4 * 56], k[:, :2 * 56], k[:, :2 * 56], off, 4, 2)):     # 8-byte base
+        with pytest.raises(_lib.MMEError):
+            bad()
+
+
+# ------------------------------------------------------------------ as they are used
+def test_graph_streams_and_two_graphs(cuda):
+    """Captured and replayed, on another stream, and two graphs of the split form that run one after the other."""
+    from mme import ops
+    g = gen(18)
+    q, k, v = make(g, 6, 6000, 8, 1, 128, cuda)
+    off = cuts([1] * 6).to(cuda)
+    koffs = [cuts(t).to(cuda) for t in ((1000,) * 6, (10, 3000, 5, 2000, 900, 85))]
+    eager = [ops.attention_docs(q, k, v, off, 8, 1, key_offsets=t, max_rows=1, causal=True, softcap=20.0) for t in koffs]
+    graphs, outs = [], []
+    for t in koffs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(ops.attention_docs(q, k, v, off, 8, 1, key_offsets=t, max_rows=1, causal=True, softcap=20.0))
+        graphs.append(graph)
+    for _ in range(4):
+        for o in outs:
+            o.zero_()
+        for graph in graphs:
+            graph.replay()
+        junk = torch.randn(1000, 1000, device=cuda) @ torch.randn(1000, 1000, device=cuda)
+        torch.cuda.synchronize()
+        assert junk.numel() and all(torch.equal(a, b) for a, b in zip(outs, eager))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = [ops.attention_docs(q, k, v, off, 8, 1, key_offsets=t, max_rows=1, causal=True, softcap=20.0) for t in koffs]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(there, eager))
+
+
+def test_a_decoder_step_over_packed_pages(cuda):
+    """q | k | v product, rotation of the q and k heads by (time, height, width), attention within each page with an
+    image prefix, output product; then a new token a page against the rotated keys kept from before."""
+    from mme import ops
+    H, hd, d = 8, 256, 512
+    pages = [(4, 6, 5), (3, 3, 8), (1, 1, 1)]  # image grid h, w, and text tokens
+    g = gen(19)
+    pos, lens, prefix = [], [], []
+    for h, w, text in pages:
+        grid = torch.stack([torch.zeros(h * w), torch.arange(h * w) // w, torch.arange(h * w) % w])
+        words = (torch.arange(text) + max(h, w)).expand(3, text)
+        pos.append(torch.cat([grid, words], 1))
+        lens.append(h * w + text)
+        prefix.append(h * w)
+    pos = torch.cat(pos, 1).to(torch.int32).contiguous()
+    x = randn(g, sum(lens), d)
+    wqkv, wo = randn(g, (H + 2) * hd, d, scale=d ** -0.5), randn(g, d, H * hd, scale=(H * hd) ** -0.5)
+    freqs, axes = ops.rope_axes_freqs((32, 48, 48), 1e4, device=cuda)
+    off, pre = cuts(lens).to(cuda), torch.tensor(prefix, dtype=torch.int32, device=cuda)
+    qkv = ops.gemm(x.to(cuda), wqkv.to(cuda))
+    plain = qkv.clone()
+    ops.rope_axes(qkv, pos.to(cuda), freqs, axes, H + 1, hd=hd, out=qkv)
+    check_rope(qkv, plain.cpu(), pos, freqs.cpu(), axes.cpu(), H + 1, hd)
+    assert torch.equal(qkv[:, (H + 1) * hd:], plain[:, (H + 1) * hd:])
+    q, k, v = qkv[:, :H * hd], qkv[:, H * hd:(H + 1) * hd], qkv[:, (H + 1) * hd:]
+    kw = dict(causal=True, prefix=pre, softcap=50.0)
+    o = ops.attention_docs(q, k, v, off, H, 1, **kw)
+    check_docs(o, q, k, v, off, H, 1, **kw)
+    y = ops.gemm(o, wo.to(cuda))
+    want = o.double().cpu() @ wo.double().t()
+    size = o.double().cpu().abs() @ wo.double().abs().t()
+    assert ((y.double().cpu() - want).abs() <= HALF * want.abs() + H * hd * 2.0 ** -24 * size).all()
+    # the last token of each page alone, against the page's keys
+    last = (off[1:] - 1).long()
+    one = cuts([1] * len(pages)).to(cuda)
+    alone = ops.attention_docs(q[last].contiguous(), k, v, one, H, 1, key_offsets=off, max_rows=1, **kw)
+    check_docs(alone, q[last], k, v, one, H, 1, key_offsets=off, **kw)
