@@ -9,22 +9,28 @@
 //
 // One workgroup = NW waves of 32 flat rows of one document and one key head, a flat row being (query, head of the
 // group), so grouped heads share the K / V tiles (and a single query fills a tile with its group's heads). Tiles of
-// 32 or 64 keys land in LDS by DMA as "chunk planes" (plane c = 16-byte column chunk c of the tile's keys, V planes
-// XOR-swizzled for the transposed reads), a ring of two, one barrier a tile. S^T = K.Q^T on 32x32x16 MFMA puts one
-// query on a lane; softmax runs in fp32 registers in one pass (running maximum, rescale only when it grows by more
-// than 2^8); P, rounded to bf16 for the matrix instruction, is directly the operand of O^T = V^T.P^T.
+// 32 or 64 keys land in LDS by DMA, row after row as they lie in memory (a wave's 1 KiB piece covers whole 128-byte
+// lines: 16-byte pieces of 64 rows made the copy the bound), a ring of two, one barrier a tile; where a row is a
+// power of two of 16-byte chunks, a chunk's place is XORed with its row so that a column of rows spreads over the
+// banks. S^T = K.Q^T on 32x32x16 MFMA puts one query on a lane; softmax runs in fp32 registers in one pass (running
+// maximum, rescale only when it grows by more than 2^8); P, rounded to bf16 for the matrix instruction, is directly
+// the operand of O^T = V^T.P^T, V^T by transposed LDS reads.
 //
-// A key outside a row's interval adds nothing to it, whatever K and V hold there: K rows past a document are never
-// read, masked scores are replaced and not added to, and a cut tile whose V holds an infinity or NaN takes a path
-// that keeps 0 x NaN out of the rows that do not see it.
+// A key outside a row's interval adds nothing to it, whatever K and V hold there: rows of another document are never
+// read, masked scores are replaced and not added to, and where a causal row comes out not finite while V holds an
+// infinity or NaN at a key that its tile has and it does not see (0 x NaN), the row is taken again from its own keys.
 //
 // Few query rows and many keys (max_rows given): the keys of each document are split into chunks, one workgroup
 // each, which leave (maximum, sum, O) in a workspace, and a second launch joins them.
+#include <type_traits>
+
 #include "common.h"
 
 #pragma clang fp contract(off)  // every fused multiply-add below is written as one
 
 namespace {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -35,8 +41,8 @@ struct DocsArgs {
     const float* slopes;
     float* part;        // split: [slot][key head][flat row] of hd + 2 floats
     long ldq, ldk, ldv, ldo;
-    long nslots;
-    int n, rows_q, rows_k, Hkv, group, hd, nch, max_rows, causal, chunk, part_rows;
+    int nslots, n, rows_q, rows_k, Hkv, group, hd, max_rows, causal, part_rows;
+    int per_log2;       // a slot's flat rows, or keys (split), are 1 << per_log2
     float scale_log2, cap_log2, cap_in;
 };
 
@@ -48,133 +54,245 @@ __device__ __forceinline__ float xsum32(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-__device__ __forceinline__ int offset_at(const int32_t* off, int i, int rows) { return min(max(off[i], 0), rows); }
-
-// Work is dealt out in slots of `per` units (flat rows, or keys). Document d owns the slots from
-// off[d] * mul / per + d on: that many always hold its units, because rounding down loses less than the one slot
-// that `+ d` adds, so a slot finds its document by a search in `off` and no table is needed. Surplus slots end at
-// once. 64 lanes look at 64 documents a step. Offsets are clamped to [0, rows]: wrong ones give wrong rows, never a
-// wrong address.
-__device__ __forceinline__ long first_slot(const int32_t* off, int d, int rows, int mul, int per) {
-    return (long)offset_at(off, d, rows) * mul / per + d;
+// 16 bytes a lane from base + off to LDS at `at` (wave-uniform, as base is) + 16 lane, retired by the caller's wait
+__device__ __forceinline__ void dma16(const char* base, unsigned off, unsigned at) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(at) : "memory", "m0");
 }
-__device__ __forceinline__ int find_doc(const int32_t* off, int n, int rows, int mul, int per, long slot) {
+__device__ __forceinline__ int clamp_row(int x, int rows) { return min(max(x, 0), rows); }
+
+// Work is dealt out in slots of `1 << sh` units (flat rows, or keys). Document d owns the slots from
+// (off[d] * mul >> sh) + d on: that many always hold its units, because rounding down loses less than the one slot
+// that `+ d` adds, so a slot finds its document by a search in `off` and no table is needed. Surplus slots end at
+// once. Offsets are clamped to [0, rows]: wrong ones give wrong rows, never a wrong address.
+__device__ __forceinline__ int first_slot(int off, int d, int mul, int sh) { return (int)(((long)off * mul >> sh) + d); }
+
+struct Doc {
+    int d, q0, qlen, k0, klen, pre, first;
+};
+template <bool SPLIT>
+__device__ __forceinline__ Doc find_doc(const DocsArgs& a, int slot) {
     const int lane = threadIdx.x & 63;
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
+    const int32_t* off = SPLIT ? a.koff : a.qoff;
+    const int rows = SPLIT ? a.rows_k : a.rows_q, mul = SPLIT ? 1 : a.group;
+    int lo = 0, hi = a.n;
+    while (hi - lo > 63) {  // 64 documents a step
         const int step = (hi - lo + 63) >> 6;
         const int i = lo + lane * step;
-        const bool le = i < hi && first_slot(off, min(i, n - 1), rows, mul, per) <= slot;
+        const bool le = i < hi && first_slot(clamp_row(off[min(i, a.n)], rows), i, mul, a.per_log2) <= slot;
         const int c = __popcll(__builtin_amdgcn_ballot_w64(le));
         if (c > 0) lo += (c - 1) * step;
         hi = min(hi, lo + step);
     }
-    return __builtin_amdgcn_readfirstlane(lo);
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    // the last step's documents: lane l holds the offsets of document lo + l, all arrays in one round trip
+    const int i = min(lo + lane, a.n);
+    const int qo = clamp_row(a.qoff[i], a.rows_q), ko = clamp_row(a.koff[i], a.rows_k);
+    const int pr = a.prefix ? a.prefix[min(i, a.n - 1)] : 0;
+    const int fs = first_slot(SPLIT ? ko : qo, i, mul, a.per_log2);
+    const int c = __popcll(__builtin_amdgcn_ballot_w64(lo + lane < hi && fs <= slot));
+    const int l = c > 0 ? c - 1 : 0;
+    Doc r;
+    r.d = lo + l;
+    r.q0 = __builtin_amdgcn_readlane(qo, l);
+    r.k0 = __builtin_amdgcn_readlane(ko, l);
+    r.qlen = max(__builtin_amdgcn_readlane(qo, l + 1) - r.q0, 0);
+    r.klen = max(__builtin_amdgcn_readlane(ko, l + 1) - r.k0, 0);
+    r.pre = min(max(__builtin_amdgcn_readlane(pr, l), 0), r.klen);
+    r.first = __builtin_amdgcn_readlane(fs, l);
+    return r;
 }
 
-template <int HDP>
+// HD: the head dim, or with GEN the least of 64, 128, 256 that holds it
+template <int HD, bool GEN>
 struct Tile {
-    static constexpr int KT = HDP > 128 ? 32 : 64;   // keys a tile: head dim 256 keeps its registers and LDS at half
+    static constexpr int KT = HD > 128 ? 32 : 64;   // keys a tile: head dim 256 keeps its registers and LDS at half
     static constexpr int KB = KT / 32;
-    static constexpr int NKS = HDP / 16;              // k-steps of Q K^T
-    static constexpr bool ONES = HDP % 32 != 0;       // a V plane of ones in the padding sums the weights
-    static constexpr int NDB = (HDP + 31) / 32;       // 32-column blocks of O^T
-    static constexpr int NKP = 2 * NKS, NVP = 4 * NDB;
-    static constexpr int PLANE = KT * 16;
-    static constexpr int BYTES = (NKP + NVP) * PLANE;
+    static constexpr int NKS = (HD + 15) / 16;        // k-steps of Q K^T
+    static constexpr int NDB = (HD + 31) / 32;        // 32-column blocks of O^T
+    // Where a row is a power of two of chunks, columns of rows would meet in the same banks: a chunk's place is XORed
+    // with bits of its row and the 1 KiB pieces (RP rows) get a gap, so that the 16 rows of a K read, and the 4 rows of
+    // a transposed V read (64 bytes each), take 256 bytes of banks between them. X is the XOR's unit in chunks: the
+    // addresses of a lane are one register for each of its NX values (and constants), not one for each k-step.
+    static constexpr bool XOR = !GEN && (HD & (HD - 1)) == 0;
+    static constexpr int KX = HD == 64 ? 2 : HD == 128 ? 4 : 8, KNX = !XOR ? 1 : HD == 256 ? 2 : 4;
+    static constexpr int VX = HD == 256 ? 8 : 4, VNX = !XOR ? 1 : HD == 128 ? 4 : 2;
+    static constexpr int KGAP = XOR ? 16 : 0, VGAP = XOR && HD == 256 ? 64 : 0;
+    static __device__ __forceinline__ int kx(int row) { return !XOR ? 0 : KX * ((HD == 64 ? row >> 1 : row) & (KNX - 1)); }
+    static __device__ __forceinline__ int vx(int row) { return !XOR ? 0 : VX * ((HD == 64 ? row >> 1 : row) & (VNX - 1)); }
+    static constexpr int NP = KT * HD / 512;           // pieces of K, and of V
+    static constexpr int VOFF = NP * (1024 + KGAP);
+    static constexpr int BYTES = VOFF + NP * (1024 + VGAP) + (HD % 32 ? 64 : 0);  // the last block reads past a row
+    // where row `row` of K or V begins (rows of a piece are contiguous); nch: chunks a row
+    static __device__ __forceinline__ int at(int row, int nch, int gap) {
+        return row * nch * 16 + (XOR ? row / (512 / HD) * gap : 0);
+    }
 };
 
-template <int HDP, int NW, int MINW, bool SPLIT>
+// One flat row from its own keys alone, [lo, hi) of its document, by one wave: 64 keys a step, a lane each for the
+// scores and a lane for each column of V (columns lane + 64 c in acc[c]); m in powers of two, weights not rounded.
+template <int HD>
+__device__ __forceinline__ void row_alone(const DocsArgs& a, const Doc& D, int gh, int kvh, int pq, int qi, int lo, int hi,
+                                       float& m, float& l, float (&acc)[(HD + 63) / 64]) {
+    const int lane = threadIdx.x & 63;
+    const bf16* q = a.q + (D.q0 + (long)qi) * a.ldq + (long)gh * a.hd;
+    const float slope = a.slopes ? a.slopes[gh] * LOG2E : 0.f;
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int c = 0; c < (HD + 63) / 64; ++c) acc[c] = 0.f;
+    for (int j0 = lo; j0 < hi; j0 += 64) {
+        const int j = j0 + lane;
+        float x = -INFINITY;
+        if (j < hi) {
+            const bf16* k = a.k + (D.k0 + (long)j) * a.ldk + (long)kvh * a.hd;
+            float s = 0.f;
+            for (int e = 0; e < a.hd; ++e) s = __builtin_fmaf(bf2f(q[e]), bf2f(k[e]), s);
+            if (a.cap_log2 != 0.f)
+                x = __builtin_fmaf(-2.0f * a.cap_log2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * a.cap_in)), a.cap_log2);
+            else
+                x = s * a.scale_log2;
+            if (a.slopes) x = __builtin_fmaf(-slope, fabsf((float)(pq - j)), x);
+        }
+        float mx = x;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
+        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
+        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        const float p = j < hi ? __builtin_amdgcn_exp2f(x - ref) : 0.f;
+        m = mn;
+        l = l * alpha + wave_sum(p);
+#pragma unroll
+        for (int c = 0; c < (HD + 63) / 64; ++c) acc[c] *= alpha;
+        for (int jj = 0; jj < min(64, hi - j0); ++jj) {
+            const float pj = __shfl(p, jj, 64);
+            const bf16* v = a.v + (D.k0 + (long)j0 + jj) * a.ldv + (long)kvh * a.hd;
+#pragma unroll
+            for (int c = 0; c < (HD + 63) / 64; ++c)
+                if (lane + 64 * c < a.hd) acc[c] = __builtin_fmaf(pj, bf2f(v[lane + 64 * c]), acc[c]);
+        }
+    }
+}
+
+// MOD: capped or biased scores
+template <int HD, bool GEN, int NW, int MINW, bool SPLIT, bool MOD>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW))) void attn_docs_kernel(DocsArgs a) {
-    using T = Tile<HDP>;
-    constexpr int KT = T::KT, KB = T::KB, NKS = T::NKS, NDB = T::NDB, PLANE = T::PLANE, QB = NW * 32;
-    __shared__ __attribute__((aligned(16))) char lds[2 * T::BYTES];
+    using T = Tile<HD, GEN>;
+    constexpr int KT = T::KT, KB = T::KB, NKS = T::NKS, NDB = T::NDB, QB = NW * 32;
+    constexpr bool HALF = GEN || HD % 16 != 0;  // the last k-step may reach past the head dim
+    constexpr int ZERO = 2 * T::BYTES;           // 16 zero bytes for it
+    __shared__ __attribute__((aligned(16))) char lds[2 * T::BYTES + (HALF ? 16 : 0)];
 
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, hh = lane >> 5;
-    long id;
+    int id;
     {  // consecutive slots of one key head (the same K / V) on one XCD
-        const long bid = blockIdx.x, nwg = gridDim.x;
-        const long xcd = bid & 7, loc = bid >> 3, q8 = nwg >> 3, r8 = nwg & 7;
+        const int bid = blockIdx.x, nwg = gridDim.x;
+        const int xcd = bid & 7, loc = bid >> 3, q8 = nwg >> 3, r8 = nwg & 7;
         id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + loc;
     }
-    const long slot = id % a.nslots;
-    const int kvh = (int)(id / a.nslots);
-    const int d = SPLIT ? find_doc(a.koff, a.n, a.rows_k, 1, a.chunk, slot) : find_doc(a.qoff, a.n, a.rows_q, a.group, QB, slot);
-    const int q0 = offset_at(a.qoff, d, a.rows_q), k0 = offset_at(a.koff, d, a.rows_k);
-    const int qlen = max(offset_at(a.qoff, d + 1, a.rows_q) - q0, 0), klen = max(offset_at(a.koff, d + 1, a.rows_k) - k0, 0);
-    const long flat = (long)min(qlen, a.max_rows) * a.group;  // flat rows of this document
-    long part = slot - (SPLIT ? first_slot(a.koff, d, a.rows_k, 1, a.chunk) : first_slot(a.qoff, d, a.rows_q, a.group, QB));
-    const long nparts = SPLIT ? ((long)klen + a.chunk - 1) / a.chunk : (flat + QB - 1) / QB;
+    const int slot = id % a.nslots, kvh = id / a.nslots;
+    const Doc D = find_doc<SPLIT>(a, slot);
+    const int qlen = D.qlen, klen = D.klen;
+    const int flat = min(qlen, a.max_rows) * a.group;  // flat rows of this document
+    int part = slot - D.first;
+    const int chunk = 1 << a.per_log2;
+    const int nparts = (int)(((SPLIT ? (long)klen : (long)flat) + chunk - 1) >> a.per_log2);
     if (part < 0 || part >= nparts || flat == 0) return;
     if (!SPLIT && a.causal) part = nparts - 1 - part;  // the rows with the most keys first
 
-    const long f0 = SPLIT ? wave * 32 : part * QB + wave * 32;
-    const long fr = f0 + r;                                     // this lane's flat row
-    const long frc = min(fr, flat - 1);
-    const int qi = (int)(frc / a.group), gh = kvh * a.group + (int)(frc % a.group);
+    const int f0 = SPLIT ? 0 : part * QB;                       // the block's first flat row
+    const int fr = f0 + wave * 32 + r;                          // this lane's
+    const int qi = min(fr, flat - 1) / a.group, gh = kvh * a.group + min(fr, flat - 1) - qi * a.group;
     const int pq = qi + klen - qlen;                            // its place among the keys
-    const int pre = a.prefix ? min(max(a.prefix[d], 0), klen) : 0;
-    const int hi = a.causal ? min(klen, max(pre, pq + 1)) : klen;  // it sees keys [0, hi)
-    const int key_lo = SPLIT ? (int)(part * a.chunk) : 0;
-    // the last row of the block sees the most keys
-    int hi_blk;
-    {
-        const int ql = (int)(min(SPLIT ? (long)QB : (part + 1) * QB, flat) - 1) / a.group;
-        hi_blk = a.causal ? min(klen, max(pre, ql + klen - qlen + 1)) : klen;
-        if (SPLIT) hi_blk = min((long)hi_blk, (long)key_lo + a.chunk);
+    const int hi = a.causal ? min(klen, max(D.pre, pq + 1)) : klen;  // it sees keys [0, hi)
+    const int key_lo = SPLIT ? part << a.per_log2 : 0;
+    // the block's first row sees the fewest keys, its last row the most
+    const int q_first = f0 / a.group, q_last = (min(f0 + QB, flat) - 1) / a.group;
+    int hi_min = a.causal ? min(klen, max(D.pre, q_first + klen - qlen + 1)) : klen;
+    int hi_max = a.causal ? min(klen, max(D.pre, q_last + klen - qlen + 1)) : klen;
+    if (SPLIT) {
+        hi_min = min((long)hi_min, (long)key_lo + chunk);
+        hi_max = min((long)hi_max, (long)key_lo + chunk);
     }
-    const int nkt = hi_blk > key_lo ? (hi_blk - key_lo + KT - 1) / KT : 0;
+    const int nfull = (hi_min - key_lo) / KT;  // tiles that every row sees whole (none where negative)
+    const int nkt = hi_max > key_lo ? (hi_max - key_lo + KT - 1) / KT : 0;
 
-    // planes past the head dim: zeros, and the ones plane at column HDP
-    for (int i = tid; i < 2 * (T::NKP + T::NVP) * KT; i += QB * 2) {
-        const int pl = i / KT % (T::NKP + T::NVP), c = pl < T::NKP ? pl : pl - T::NKP;
-        if (c < a.nch) continue;
-        const unsigned short one = (T::ONES && pl >= T::NKP && c == HDP / 8) ? 0x3F80 : 0;
-        *reinterpret_cast<u16x8*>(lds + (long)i * 16) = u16x8{one, one, one, one, one, one, one, one};
-    }
+    const int nch = GEN ? a.hd >> 3 : HD / 8;  // 16-byte chunks a row, in memory and in LDS
+    if (HALF && tid == 0) *reinterpret_cast<u16x8*>(lds + ZERO) = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+
+    const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS char*)lds;
+    const char* kbase = (const char*)(a.k + (D.k0 + (long)key_lo) * a.ldk + (long)kvh * a.hd);
+    const char* vbase = (const char*)(a.v + (D.k0 + (long)key_lo) * a.ldv + (long)kvh * a.hd);
+    // piece idx of K's, then of V's nch * KT / 64: LDS chunks 64 idx .. + 63, i.e. chunk c of row (64 idx + lane) / nch.
+    // A lane's places in the pieces are the same in every tile but one that reaches past the document.
+    const int npc = nch * KT / 64;
+    constexpr int PIECES = (HD / 8 * KT / 64 * 2 + NW - 1) / NW;
+    auto place = [&](int i, int most) __attribute__((always_inline)) {
+        const int idx = wave + NW * i, pc = idx >= npc ? idx - npc : idx;
+        const int row = (pc * 64 + lane) / nch, ch = pc * 64 + lane - row * nch;
+        return idx >= npc ? (unsigned)min(row, most) * (unsigned)(2 * a.ldv) + (ch ^ T::vx(row)) * 16
+                          : (unsigned)min(row, most) * (unsigned)(2 * a.ldk) + (ch ^ T::kx(row)) * 16;
+    };
+    unsigned at[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) at[i] = place(i, KT);
+    auto issue = [&](int t, unsigned so) __attribute__((always_inline)) {
+        const char *kt = kbase + (long)t * KT * 2 * a.ldk, *vt = vbase + (long)t * KT * 2 * a.ldv;
+        const int most = klen - 1 - key_lo - t * KT;
+        auto piece = [&](int i, unsigned from) __attribute__((always_inline)) {
+            const int idx = wave + NW * i;
+            const bool isV = idx >= npc;
+            const unsigned to = isV ? T::VOFF + (idx - npc) * (1024 + T::VGAP) : idx * (1024 + T::KGAP);
+            dma16(isV ? vt : kt, from, lds0 + so + to);
+        };
+        if (most >= KT - 1) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+                if (wave + NW * i < 2 * npc) piece(i, at[i]);
+        } else {
+#pragma unroll 1
+            for (int i = 0; wave + NW * i < 2 * npc; ++i) piece(i, place(i, most));
+        }
+    };
+    if (nkt > 0) issue(0, 0);
 
     bf16x8 qf[NKS];  // B operand: Q^T[16 ks + 8 hh + j][row r]
     {
-        const bf16* qrow = a.q + (q0 + (long)qi) * a.ldq + (long)gh * a.hd;
+        const bf16* qrow = a.q + (D.q0 + (long)qi) * a.ldq + (long)gh * a.hd;
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks)
-            qf[ks] = __builtin_bit_cast(bf16x8, load_chunk_or_zero(qrow, 2 * ks + hh, a.nch));
+            qf[ks] = HALF ? __builtin_bit_cast(bf16x8, load_chunk_or_zero(qrow, 2 * ks + hh, nch))
+                          : *reinterpret_cast<const bf16x8*>(qrow + (2 * ks + hh) * 8);
     }
-    const float slope = a.slopes ? a.slopes[gh] * LOG2E : 0.f;
-    const float c = a.cap_log2 != 0.f || a.slopes ? 1.0f : a.scale_log2;  // what a score is still multiplied by
+    const float slope = MOD && a.slopes ? a.slopes[gh] * LOG2E : 0.f;
+    const float c = MOD ? 1.0f : a.scale_log2;  // what a score is still multiplied by
 
-    const bf16* kbase = a.k + (long)k0 * a.ldk + (long)kvh * a.hd;
-    const bf16* vbase = a.v + (long)k0 * a.ldv + (long)kvh * a.hd;
-    const int nins = a.nch * 2 * KT / 64;  // DMA instructions a tile: KT 64 one plane each, KT 32 two
-    auto issue = [&](int t, unsigned so) {
-        for (int idx = wave; idx < nins; idx += NW) {
-            const int plane = KT == 64 ? idx : 2 * idx + hh;
-            const int first = KT == 64 ? idx : 2 * idx;
-            const bool isV = first >= a.nch;
-            const int cc = isV ? plane - a.nch : plane;
-            const int kl = lane & (KT - 1);
-            const int key = min(key_lo + t * KT + (isV ? kl ^ (4 * (cc & 3)) : kl), klen - 1);
-            const bf16* src = isV ? vbase + (long)key * a.ldv + cc * 8 : kbase + (long)key * a.ldk + cc * 8;
-            glds16_asm(src, lds + so + (isV ? T::NKP + first - a.nch : first) * PLANE);
-        }
+    unsigned ka[T::KNX];
+#pragma unroll
+    for (int g = 0; g < T::KNX; ++g) ka[g] = lds0 + T::at(r, nch, T::KGAP) + (((g * T::KX) ^ T::kx(r)) + hh) * 16;
+    auto kfrag = [&](unsigned so, int kb, int ks) __attribute__((always_inline)) {
+        constexpr int U = T::KX / 2, W = T::KNX * U;  // k-steps a unit, and all units
+        unsigned at = (T::XOR ? ka[ks / U % T::KNX] + (ks % U + ks / W * W) * 32 : ka[0] + ks * 32) + so +
+                      kb * T::at(32, nch, T::KGAP);
+        if (HALF && (GEN || ks == NKS - 1)) at = 2 * ks + hh < nch ? at : lds0 + ZERO;
+        return *reinterpret_cast<const LDS_AS bf16x8*>((uintptr_t)at);
     };
-
-    const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS char*)lds;
-    const unsigned kb0 = lds0 + hh * PLANE + r * 16;
-    unsigned vbj[2];  // V^T fragment: two transposed reads, keys 16 s + 8 j + 4 hh + q at columns 16 half + 4 p ..
+    // V^T fragment of key step i: two transposed reads, keys 16 i + 8 j + 4 hh + q at columns 32 db + 16 half + 4 p ..
+    unsigned va[T::VNX];
     {
         const int i16 = lane & 15, q = i16 >> 2, p = i16 & 3, half = (lane >> 4) & 1;
-        const int cc = 2 * half + (p >> 1);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-            vbj[j] = lds0 + (T::NKP + cc) * PLANE + (((8 * j + 4 * hh + q) ^ (4 * cc)) * 16) + (p & 1) * 8;
+        for (int g = 0; g < T::VNX; ++g)
+            va[g] = lds0 + T::VOFF + T::at(4 * hh + q, nch, T::VGAP) + (((g * T::VX) ^ T::vx(q)) + 2 * half + (p >> 1)) * 16 +
+                    (p & 1) * 8;
     }
-    auto vfrag = [&](unsigned so, int i, int db) __attribute__((always_inline)) {  // key step i = 2 kb + s
-        const unsigned off = so + db * 4 * PLANE + i * 256;
-        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(uintptr_t)(vbj[0] + off));
-        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(uintptr_t)(vbj[1] + off));
+    auto vfrag = [&](unsigned so, int i, int db) __attribute__((always_inline)) {
+        constexpr int U = T::VX / 4, W = T::VNX * U;
+        const unsigned at = (T::XOR ? va[db / U % T::VNX] + (db % U + db / W * W) * 64 : va[0] + db * 64) + so +
+                            i * T::at(16, nch, T::VGAP);
+        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(uintptr_t)at);
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(uintptr_t)(at + T::at(8, nch, T::VGAP)));
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
@@ -185,7 +303,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
     float m = -INFINITY, lsum = 0.f;
 
-    auto tile = [&](int t, const unsigned so) __attribute__((always_inline)) {
+    // CUT: some row may not see all of the tile's keys
+    auto tile = [&](auto cut_c, int t, const unsigned so) __attribute__((always_inline)) {
+        constexpr bool CUT = decltype(cut_c)::value;
         const int key0 = key_lo + t * KT;
         f32x16 sc[KB];
 #pragma unroll
@@ -194,14 +314,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
 #pragma unroll
             for (int e = 0; e < 16; ++e) z[e] = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) {
-                const bf16x8 kf = *reinterpret_cast<const LDS_AS bf16x8*>((uintptr_t)(kb0 + so + kb * 512 + ks * 2 * PLANE));
-                z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[ks], z, 0, 0, 0);
+            for (int ks = 0; ks < NKS; ++ks)
+            {
+                if (!GEN || 2 * ks < nch) z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfrag(so, kb, ks), qf[ks], z, 0, 0, 0);
+                if (HD > 128 && ks % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
             sc[kb] = z;
         }
         // register e of block kb scores key key0 + 32 kb + (e & 3) + 8 (e >> 2) + 4 hh
-        if (a.cap_log2 != 0.f) {  // cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)), log2(e) folded in
+        if (MOD && a.cap_log2 != 0.f) {  // cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)), log2(e) folded in
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -209,13 +330,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
                     const float w = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[kb][e] * a.cap_in));
                     sc[kb][e] = __builtin_fmaf(-2.0f * a.cap_log2, w, a.cap_log2);
                 }
-        } else if (a.slopes) {
+        } else if (MOD) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sc[kb][e] *= a.scale_log2;
         }
-        if (a.slopes) {
+        if (MOD && a.slopes) {
             const float db = (float)(pq - key0 - 4 * hh);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
@@ -223,14 +344,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
                 for (int e = 0; e < 16; ++e)
                     sc[kb][e] = __builtin_fmaf(-slope, fabsf(db - (float)(32 * kb + (e & 3) + 8 * (e >> 2))), sc[kb][e]);
         }
-        const int lim = hi - key0;
-        const bool cut = __builtin_amdgcn_ballot_w64(lim < KT) != 0;
-        if (cut) {
+        const int lim = hi - key0 - 4 * hh;
+        if (CUT) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (32 * kb + (e & 3) + 8 * (e >> 2) + 4 * hh >= lim) sc[kb][e] = -INFINITY;
+                    if (32 * kb + (e & 3) + 8 * (e >> 2) >= lim) sc[kb][e] = -INFINITY;
         }
 
         float mloc = fmaxf(sc[0][0], sc[0][1]);
@@ -244,7 +364,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
         if (__builtin_amdgcn_ballot_w64((mloc - m) * c > 8.0f)) {  // P stays under 2^8 otherwise
             const float mnew = fmaxf(m, mloc);
             const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mnew) * c);
-            if (!T::ONES) lsum *= alpha;
+            lsum *= alpha;
 #pragma unroll
             for (int i = 0; i < NDB; ++i) o[i] *= alpha;
             m = mnew;
@@ -261,56 +381,30 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
             cf = 1.0f;
         }
         bf16x8 pk[2 * KB];
-        float psum = 0.f;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][e], cf, -mc));
-                if (!T::ONES) psum += p;
-                pk[2 * kb + (e >> 3)][e & 7] = f2bf(p);
-            }
-        if (!T::ONES) lsum += psum;
+            for (int e = 0; e < 16; ++e)
+                pk[2 * kb + (e >> 3)][e & 7] = f2bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][e], cf, -mc)));
+        // the rounded weights are summed: where one weight is nearly all, its rounding divides out
+        float psum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * KB; ++i) {
+            const bf16x2 one = {1.0f, 1.0f};
+            psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 0, 1), one, psum, false);
+            psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 2, 3), one, psum, false);
+            psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 4, 5), one, psum, false);
+            psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 6, 7), one, psum, false);
+        }
+        lsum += psum;
 
-        bool odd = false;
-        if (cut) {  // does V of this tile hold an infinity or NaN?
-            u16x4 least = {0xffff, 0xffff, 0xffff, 0xffff};
 #pragma unroll
-            for (int i = 0; i < 2 * KB; ++i)
+        for (int i = 0; i < 2 * KB; ++i)
 #pragma unroll
-                for (int db = 0; db < NDB; ++db) {
-                    const u16x8 w = ~__builtin_bit_cast(u16x8, vfrag(so, i, db)) & (unsigned short)0x7f80;
-                    least = __builtin_elementwise_min(least, __builtin_elementwise_min(
-                        __builtin_shufflevector(w, w, 0, 1, 2, 3), __builtin_shufflevector(w, w, 4, 5, 6, 7)));
-                }
-            const bool bad = least[0] == 0 || least[1] == 0 || least[2] == 0 || least[3] == 0;
-            odd = __builtin_amdgcn_ballot_w64(bad) != 0;
-        }
-        if (!odd) {
-#pragma unroll
-            for (int i = 0; i < 2 * KB; ++i)
-#pragma unroll
-                for (int db = 0; db < NDB; ++db)
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfrag(so, i, db), pk[i], o[db], 0, 0, 0);
-        } else {  // key by key, a row that does not see the key keeping what it had
-#pragma unroll
-            for (int i = 0; i < 2 * KB; ++i)
-                for (int kk = 0; kk < 16; ++kk) {  // element kk & 7 of lane half kk >> 3
-                    const int j = kk & 7, h1 = kk >> 3;
-                    const bool sees = 16 * i + (j & 3) + 8 * (j >> 2) + 4 * h1 < lim;
-                    u32x4 keep;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) keep[w] = (hh == h1 && (j >> 1) == w) ? 0xffffu << (16 * (j & 1)) : 0u;
-                    const bf16x8 p1 = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, pk[i]) & keep);
-#pragma unroll
-                    for (int db = 0; db < NDB; ++db) {
-                        const bf16x8 v1 = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, vfrag(so, i, db)) & keep);
-                        const f32x16 s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v1, p1, o[db], 0, 0, 0);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[db][e] = sees ? s[e] : o[db][e];
-                    }
-                }
-        }
+            for (int db = 0; db < NDB; ++db) {
+                o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfrag(so, i, db), pk[i], o[db], 0, 0, 0);
+                if (HD > 128 && db % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            }
     };
 
     // this wave's part of the next tile has landed and its LDS reads are done; then everybody's
@@ -319,22 +413,28 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    if (nkt > 0) issue(0, 0);
-    for (int t = 0; t < nkt; t += 2) {
+    if (NW > 4 && wave >= NW / 2) __builtin_amdgcn_s_setprio(1);  // PRIO
+    int t = 0;
+    for (; t + 1 < nfull; t += 2) {  // two a turn: the ring's slots are constants
         meet();
-        if (t + 1 < nkt) issue(t + 1, T::BYTES);
-        tile(t, 0);
-        if (t + 1 < nkt) {
-            meet();
-            if (t + 2 < nkt) issue(t + 2, 0);
-            tile(t + 1, T::BYTES);
-        }
+        issue(t + 1, T::BYTES);
+        tile(std::false_type{}, t, 0);
+        meet();
+        if (t + 2 < nkt) issue(t + 2, 0);
+        tile(std::false_type{}, t + 1, T::BYTES);
+    }
+    for (; t < nkt; ++t) {
+        const unsigned so = t & 1 ? T::BYTES : 0;
+        meet();
+        if (t + 1 < nkt) issue(t + 1, T::BYTES - so);
+        if (__builtin_amdgcn_ballot_w64(hi > key_lo + t * KT)) tile(std::true_type{}, t, so);
     }
 
-    const float l = T::ONES ? o[HDP / 32][4 * ((HDP % 32) / 8)] : xsum32(lsum);
+    const float l = xsum32(lsum);
+    const float inv = hi > 0 ? 1.0f / l : 0.f;  // a row that sees nothing is 0
     if constexpr (SPLIT) {
         if (fr < flat) {
-            float* row = a.part + ((slot * a.Hkv + kvh) * a.part_rows + fr) * (a.hd + 2);
+            float* row = a.part + (((long)slot * a.Hkv + kvh) * a.part_rows + fr) * (a.hd + 2);
             if (hh == 0) *reinterpret_cast<float2*>(row) = make_float2(m * c, l);
 #pragma unroll
             for (int db = 0; db < NDB; ++db)
@@ -347,46 +447,87 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
                     }
                 }
         }
-        return;
+    } else {
+        bf16* orow = a.out + (D.q0 + (long)qi) * a.ldo + (long)gh * a.hd;
+        // registers 4 mm .. of block db = columns 32 db + 8 mm + 4 hh ..; the swap of the lane halves makes 16 bytes
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+            for (int mm = 0; mm < 4; mm += 2) {
+                bf16x4 v0, v1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v0[e] = f2bf(o[db][4 * mm + e] * inv);
+                    v1[e] = f2bf(o[db][4 * mm + 4 + e] * inv);
+                }
+                const uint2 x = __builtin_bit_cast(uint2, v0), y = __builtin_bit_cast(uint2, v1);
+                const auto sx = __builtin_amdgcn_permlane32_swap(x.x, y.x, false, false);
+                const auto sy = __builtin_amdgcn_permlane32_swap(x.y, y.y, false, false);
+                const int d0 = 32 * db + 8 * (mm + hh);
+                if (fr < flat && d0 < a.hd) *reinterpret_cast<uint4*>(orow + d0) = make_uint4(sx[0], sy[0], sx[1], sy[1]);
+            }
     }
-    const float inv = hi > 0 ? 1.0f / l : 0.f;  // a row that sees nothing is 0
-    bf16* orow = a.out + (q0 + (long)qi) * a.ldo + (long)gh * a.hd;
-    // registers 4 mm .. of block db = columns 32 db + 8 mm + 4 hh ..; the swap of the lane halves makes 16 bytes
+    if (!a.causal) return;  // all rows saw the same keys; what the last tile had besides repeats the last of them
+
+    float nan = 0.f;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int mm = 0; mm < 4; mm += 2) {
-            bf16x4 v0, v1;
+        for (int e = 0; e < 16; ++e)
+            if (32 * db + 8 * (e >> 2) < HD) nan = __builtin_fmaf(o[db][e], 0.f, nan);
+    unsigned long bad = __builtin_amdgcn_ballot_w64(fr < flat && nan != 0.f);
+    bad = (bad | bad >> 32) & 0xffffffffu;
+    if (bad == 0) return;
+    // keys that this wave's tiles had and some of its rows do not see: does V hold an infinity or NaN there?
+    bool found = false;
+    {
+        int least = hi, most = hi;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v0[e] = f2bf(o[db][4 * mm + e] * inv);
-                v1[e] = f2bf(o[db][4 * mm + 4 + e] * inv);
-            }
-            const uint2 x = __builtin_bit_cast(uint2, v0), y = __builtin_bit_cast(uint2, v1);
-            const auto sx = __builtin_amdgcn_permlane32_swap(x.x, y.x, false, false);
-            const auto sy = __builtin_amdgcn_permlane32_swap(x.y, y.y, false, false);
-            const int d0 = 32 * db + 8 * (mm + hh);
-            if (fr < flat && d0 < a.hd) *reinterpret_cast<uint4*>(orow + d0) = make_uint4(sx[0], sy[0], sx[1], sy[1]);
+        for (int x = 16; x > 0; x >>= 1) least = min(least, __shfl_xor(least, x, 64)), most = max(most, __shfl_xor(most, x, 64));
+        const int end = min(klen, key_lo + (max(most - key_lo, 0) + KT - 1) / KT * KT);
+        for (int j = max(least, key_lo); j < end; ++j) {
+            const bf16* v = a.v + (D.k0 + (long)j) * a.ldv + (long)kvh * a.hd;
+            for (int e = lane; e < a.hd; e += 64) found |= !(fabsf(bf2f(v[e])) < INFINITY);
         }
+    }
+    if (__builtin_amdgcn_ballot_w64(found) == 0) return;
+    for (int x = 0; x < 32; ++x) {
+        if (!(bad >> x & 1)) continue;
+        const int fx = f0 + wave * 32 + x, qx = fx / a.group, gx = kvh * a.group + fx - qx * a.group, px = qx + klen - qlen;
+        const int hx = min(klen, max(D.pre, px + 1));
+        float mx, lx, acc[(HD + 63) / 64];
+        row_alone<HD>(a, D, gx, kvh, px, qx, key_lo, SPLIT ? (int)min((long)hx, (long)key_lo + chunk) : hx, mx, lx, acc);
+        float* row = SPLIT ? a.part + (((long)slot * a.Hkv + kvh) * a.part_rows + fx) * (a.hd + 2) : nullptr;
+        if (SPLIT && lane == 0) row[0] = mx, row[1] = lx;
+#pragma unroll
+        for (int cc = 0; cc < (HD + 63) / 64; ++cc) {
+            const int e = lane + 64 * cc;
+            if (e >= a.hd) continue;
+            if (SPLIT)
+                row[2 + e] = acc[cc];
+            else
+                a.out[(D.q0 + (long)qx) * a.ldo + (long)gx * a.hd + e] = f2bf(hx > 0 ? acc[cc] / lx : 0.f);
+        }
+    }
 }
 
 // Joins a document's chunks: one wave a (document, flat row, key head), 64 columns a step.
 __global__ __launch_bounds__(256) void join_docs_kernel(DocsArgs a) {
     const int lane = threadIdx.x & 63;
     const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const long fr = w % a.part_rows;
+    const int fr = (int)(w % a.part_rows);
     const int kvh = (int)(w / a.part_rows % a.Hkv);
     const int d = (int)(w / a.part_rows / a.Hkv);
     if (d >= a.n) return;
-    const int q0 = offset_at(a.qoff, d, a.rows_q), k0 = offset_at(a.koff, d, a.rows_k);
-    const int qlen = max(offset_at(a.qoff, d + 1, a.rows_q) - q0, 0), klen = max(offset_at(a.koff, d + 1, a.rows_k) - k0, 0);
-    if (fr >= (long)min(qlen, a.max_rows) * a.group) return;
-    const int qi = (int)(fr / a.group), gh = kvh * a.group + (int)(fr % a.group);
+    const int q0 = clamp_row(a.qoff[d], a.rows_q), k0 = clamp_row(a.koff[d], a.rows_k);
+    const int qlen = max(clamp_row(a.qoff[d + 1], a.rows_q) - q0, 0), klen = max(clamp_row(a.koff[d + 1], a.rows_k) - k0, 0);
+    if (fr >= min(qlen, a.max_rows) * a.group) return;
+    const int qi = fr / a.group, gh = kvh * a.group + fr % a.group;
     const int pre = a.prefix ? min(max(a.prefix[d], 0), klen) : 0;
     const int hi = a.causal ? min(klen, max(pre, qi + klen - qlen + 1)) : klen;
-    const int nparts = (int)(((long)klen + a.chunk - 1) / a.chunk);
+    const int nparts = (int)(((long)klen + (1 << a.per_log2) - 1) >> a.per_log2);
     const long step = (long)a.Hkv * a.part_rows * (a.hd + 2);
-    const float* p0 = a.part + ((first_slot(a.koff, d, a.rows_k, 1, a.chunk) * a.Hkv + kvh) * a.part_rows + fr) * (a.hd + 2);
+    const float* p0 = a.part + (((long)first_slot(k0, d, 1, a.per_log2) * a.Hkv + kvh) * a.part_rows + fr) * (a.hd + 2);
     float m = -INFINITY;
     for (int s = lane; s < nparts; s += 64) m = fmaxf(m, p0[s * step]);
 #pragma unroll
@@ -405,46 +546,51 @@ __global__ __launch_bounds__(256) void join_docs_kernel(DocsArgs a) {
 
 struct Plan {
     bool split;
-    int NW, chunk, part_rows;
-    long nslots;
+    int NW, per_log2, part_rows, nslots;
     size_t ws;
 };
 
-int padded(int hd) { return hd <= 64 ? 64 : hd <= 80 ? 80 : hd <= 128 ? 128 : 256; }
+constexpr int NWL = 8, MINW1 = 1;
 
 Plan make_plan(int n, int rows_q, int rows_k, int Hkv, int group, int hd, int max_rows) {
     Plan p{};
     const long mean = n ? (long)rows_q * group / n : 0;
-    p.NW = mean <= 48 ? 1 : 4;
-    p.nslots = (long)rows_q * group / (p.NW * 32) + n;
+    p.NW = mean <= 48 ? 1 : NWL;
+    p.per_log2 = p.NW == 1 ? 5 : 8;
+    long nslots = ((long)rows_q * group >> p.per_log2) + n;
     const long mr = (long)max_rows * group;
-    const long blocks = p.nslots * Hkv;
+    const long blocks = nslots * Hkv;
     if (n && mr <= 32 && rows_k / n > 256 && blocks < 2048) {
         p.split = true;
         p.NW = 1;
         const long want = (2048 + Hkv - 1) / Hkv;  // chunks in all
-        long chunk = ((long)rows_k / want + 63) / 64 * 64;
-        p.chunk = (int)(chunk < 128 ? 128 : chunk);
+        p.per_log2 = 7;
+        while (((long)rows_k >> p.per_log2) > want) ++p.per_log2;
         p.part_rows = (int)mr;
-        p.nslots = (long)rows_k / p.chunk + n;
-        p.ws = (size_t)p.nslots * Hkv * mr * (hd + 2) * 4;
+        nslots = ((long)rows_k >> p.per_log2) + n;
+        p.ws = (size_t)nslots * Hkv * mr * (hd + 2) * 4;
     }
+    p.nslots = nslots * Hkv < (1L << 31) ? (int)nslots : -1;
     return p;
 }
 
-template <int HDP, int NW, int MINW, bool SPLIT>
+template <int HD, bool GEN, int NW, int MINW, bool SPLIT>
 void launch_docs(const DocsArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL((attn_docs_kernel<HDP, NW, MINW, SPLIT>), dim3((unsigned)(a.nslots * a.Hkv)), dim3(NW * 64), 0, s, a);
+    const dim3 grid((unsigned)(a.nslots * a.Hkv)), block(NW * 64);
+    if (a.cap_log2 != 0.f || a.slopes)
+        hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, SPLIT, true>), grid, block, 0, s, a);
+    else
+        hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, SPLIT, false>), grid, block, 0, s, a);
 }
 
-template <int HDP, int MINW>
+template <int HD, bool GEN, int MINW>
 void launch_width(const DocsArgs& a, const Plan& p, hipStream_t s) {
     if (p.split)
-        launch_docs<HDP, 1, MINW, true>(a, s);
+        launch_docs<HD, GEN, 1, MINW1, true>(a, s);
     else if (p.NW == 1)
-        launch_docs<HDP, 1, MINW, false>(a, s);
+        launch_docs<HD, GEN, 1, MINW1, false>(a, s);
     else
-        launch_docs<HDP, 4, MINW, false>(a, s);
+        launch_docs<HD, GEN, NWL, MINW, false>(a, s);
 }
 
 int check_docs(int n, int rows_q, int rows_k, int Hq, int Hkv, int hd, int max_rows) {
@@ -476,30 +622,40 @@ extern "C" int mme_attention_docs(const void* q, long ldq, const void* k, long l
     MME_REQUIRE(ldq % 8 == 0 && ldk % 8 == 0 && ldv % 8 == 0 && ldo % 8 == 0 && ldq >= (long)Hq * hd &&
                     ldo >= (long)Hq * hd && ldk >= (long)Hkv * hd && ldv >= (long)Hkv * hd,
                 "mme_attention_docs: bad leading dims");
+    MME_REQUIRE(ldk < (1L << 24) && ldv < (1L << 24), "mme_attention_docs: leading dims of k and v must be under 2^24");
     MME_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0 &&
                     (((uintptr_t)q_offsets | (uintptr_t)k_offsets | (uintptr_t)prefix | (uintptr_t)slopes) & 3) == 0,
                 "mme_attention_docs: misaligned pointer");
     const int mr = max_rows < rows_q ? max_rows : rows_q;
     if (mr == 0) return MME_OK;
     const Plan p = make_plan(n, rows_q, rows_k, Hkv, Hq / Hkv, hd, mr);
-    MME_REQUIRE(p.nslots * Hkv < (1L << 31) && (long)n * Hkv * p.part_rows < (1L << 33), "mme_attention_docs: too many rows");
+    MME_REQUIRE(p.nslots >= 0 && (long)rows_q * (Hq / Hkv) < (1L << 31) - 512 && (long)n * Hkv * p.part_rows < (1L << 33),
+                "mme_attention_docs: too many rows");
     MME_REQUIRE(p.ws == 0 || (workspace && ws_bytes >= p.ws && ((uintptr_t)workspace & 15) == 0),
                 "mme_attention_docs: workspace of %zu bytes, %zu needed", ws_bytes, p.ws);
     DocsArgs a{};
     a.q = (const bf16*)q, a.k = (const bf16*)k, a.v = (const bf16*)v, a.out = (bf16*)out;
     a.qoff = q_offsets, a.koff = k_offsets, a.prefix = prefix, a.slopes = slopes, a.part = (float*)workspace;
     a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldo = ldo, a.nslots = p.nslots;
-    a.n = n, a.rows_q = rows_q, a.rows_k = rows_k, a.Hkv = Hkv, a.group = Hq / Hkv, a.hd = hd, a.nch = hd / 8;
-    a.max_rows = mr, a.causal = causal ? 1 : 0, a.chunk = p.chunk, a.part_rows = p.part_rows;
+    a.n = n, a.rows_q = rows_q, a.rows_k = rows_k, a.Hkv = Hkv, a.group = Hq / Hkv, a.hd = hd;
+    a.max_rows = mr, a.causal = causal ? 1 : 0, a.per_log2 = p.per_log2, a.part_rows = p.part_rows;
     a.scale_log2 = scale * LOG2E;
     a.cap_log2 = softcap * LOG2E;
     a.cap_in = softcap != 0.f ? 2.0f * a.scale_log2 / softcap : 0.f;
     hipStream_t s = as_stream(stream);
-    switch (padded(hd)) {
-        case 64: launch_width<64, 2>(a, p, s); break;
-        case 80: launch_width<80, 2>(a, p, s); break;
-        case 128: launch_width<128, 2>(a, p, s); break;
-        default: launch_width<256, 1>(a, p, s); break;
+    switch (hd) {
+        case 64: launch_width<64, false, 3>(a, p, s); break;
+        case 72: launch_width<72, false, 3>(a, p, s); break;
+        case 80: launch_width<80, false, 3>(a, p, s); break;
+        case 128: launch_width<128, false, 2>(a, p, s); break;
+        case 256: launch_width<256, false, 2>(a, p, s); break;
+        default:
+            if (hd < 64)
+                launch_width<64, true, 2>(a, p, s);
+            else if (hd < 128)
+                launch_width<128, true, 2>(a, p, s);
+            else
+                launch_width<256, true, 1>(a, p, s);
     }
     if (p.split) {
         if (int rc = mme_check_launch("mme_attention_docs")) return rc;

@@ -125,7 +125,7 @@ def cuts(lens, first=0):
     return torch.tensor(np.concatenate([[0], np.cumsum(lens)]) + first, dtype=torch.int32)
 
 
-def check_docs(got, q, k, v, offsets, heads, kv_heads, **kw):
+def check_docs(got, q, k, v, offsets, heads, kv_heads, rows=slice(None), **kw):
     f = lambda t: None if t is None else t.double().cpu().numpy() if t.is_floating_point() else t.cpu().numpy()  # noqa: E731
     kw = {n: f(t) if isinstance(t, torch.Tensor) else t for n, t in kw.items()}
     want, spread, reach = oracle.attention_docs(f(q), f(k), f(v), f(offsets), heads, kv_heads, **kw)
@@ -137,6 +137,7 @@ def check_docs(got, q, k, v, offsets, heads, kv_heads, **kw):
     delta = (hd + 4) * 2.0 ** -24 * np.repeat(reach, hd, 1) + 3 * kw.get("softcap", 0.0) * 2.0 ** -23 + 2.0 ** -20
     tol = HALF * (spread + 2 * np.abs(want)) + 2 * (spread + np.abs(want)) * delta
     tol += want.shape[0] * 2.0 ** -24 * spread
+    got, want, tol = got[rows], want[rows], tol[rows]
     bad = ~(np.abs(got - want) <= tol)
     assert not bad.any(), (np.argwhere(bad)[:5], got[bad][:5], want[bad][:5], tol[bad][:5])
 
@@ -253,16 +254,12 @@ def test_docs_what_masked_keys_hold_does_not_matter(cuda, hd, value):
     bad = np.zeros(200, bool)
     bad[2 + 70 + 41:2 + 160] = True
     got = ops.attention_docs(q, k, v, off, 2, 1, causal=True)
-    clean_k, clean_v = k.clone(), v.clone()
-    for t in (clean_k, clean_v):
-        t[~torch.isfinite(t)] = 0
-    clean = ops.attention_docs(q, clean_k, clean_v, off, 2, 1, causal=True)
     inside = np.zeros(200, bool)
     inside[2:195] = True
     good = torch.from_numpy(inside & ~bad).to(cuda)
     assert torch.isfinite(got[good].float()).all()
-    # the odd path adds key by key: the same fp32 sums in another order
-    assert torch.allclose(got[good].float(), clean[good].float(), rtol=2 * HALF, atol=2.0 ** -16)
+    # rows that are taken again have weights that are not rounded, which the bound of rounded ones holds as well
+    check_docs(got, q, k, v, off, 2, 1, causal=True, rows=inside & ~bad)
     if value != value:
         assert torch.isnan(got[2 + 70 + 41:2 + 160].float()).all()
 
