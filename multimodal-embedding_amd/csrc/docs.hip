@@ -39,7 +39,7 @@ struct DocsArgs {
     bf16* out;
     const int32_t *qoff, *koff, *prefix;
     const float* slopes;
-    float* part;        // split: [slot][key head][flat row] of hd + 2 floats
+    float *part, *stat;  // split: O [slot][key head][flat row][hd], and (maximum, sum) [slot][key head][flat row][2]
     long ldq, ldk, ldv, ldo;
     int nslots, n, rows_q, rows_k, Hkv, group, hd, max_rows, causal, part_rows;
     int per_log2;       // a slot's flat rows, or keys (split), are 1 << per_log2
@@ -173,8 +173,8 @@ __device__ __forceinline__ void row_alone(const DocsArgs& a, const Doc& D, int g
     }
 }
 
-// MOD: capped or biased scores
-template <int HD, bool GEN, int NW, int MINW, bool SPLIT, bool MOD>
+// MODE: 1 = capped scores, 2 = biased by distance, 3 = both
+template <int HD, bool GEN, int NW, int MINW, bool SPLIT, int MODE>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW))) void attn_docs_kernel(DocsArgs a) {
     using T = Tile<HD, GEN>;
     constexpr int KT = T::KT, KB = T::KB, NKS = T::NKS, NDB = T::NDB, QB = NW * 32;
@@ -186,12 +186,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, hh = lane >> 5;
     int id;
-    {  // consecutive slots of one key head (the same K / V) on one XCD
+    {  // consecutive work on one XCD: slots of one key head (the same K / V)
         const int bid = blockIdx.x, nwg = gridDim.x;
         const int xcd = bid & 7, loc = bid >> 3, q8 = nwg >> 3, r8 = nwg & 7;
         id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + loc;
     }
-    const int slot = id % a.nslots, kvh = id / a.nslots;
+    // where the K / V of a slot are its own, the key heads go side by side, as their rows lie in shared lines
+    constexpr bool OWN = SPLIT || NW == 1;
+    const int slot = OWN ? id / a.Hkv : id % a.nslots, kvh = OWN ? id % a.Hkv : id / a.nslots;
     const Doc D = find_doc<SPLIT>(a, slot);
     const int qlen = D.qlen, klen = D.klen;
     const int flat = min(qlen, a.max_rows) * a.group;  // flat rows of this document
@@ -224,38 +226,33 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS char*)lds;
     const char* kbase = (const char*)(a.k + (D.k0 + (long)key_lo) * a.ldk + (long)kvh * a.hd);
     const char* vbase = (const char*)(a.v + (D.k0 + (long)key_lo) * a.ldv + (long)kvh * a.hd);
-    // piece idx of K's, then of V's nch * KT / 64: LDS chunks 64 idx .. + 63, i.e. chunk c of row (64 idx + lane) / nch.
-    // A lane's places in the pieces are the same in every tile but one that reaches past the document.
+    // a tile of K (or V) is nch * KT / 64 pieces; piece p: LDS chunks 64 p .. + 63, chunk c of row (64 p + lane) / nch.
+    // A lane's places in them are the same in every tile but one that reaches past the document.
     const int npc = nch * KT / 64;
-    constexpr int PIECES = (HD / 8 * KT / 64 * 2 + NW - 1) / NW;
-    auto place = [&](int i, int most) __attribute__((always_inline)) {
-        const int idx = wave + NW * i, pc = idx >= npc ? idx - npc : idx;
-        const int row = (pc * 64 + lane) / nch, ch = pc * 64 + lane - row * nch;
-        return idx >= npc ? (unsigned)min(row, most) * (unsigned)(2 * a.ldv) + (ch ^ T::vx(row)) * 16
-                          : (unsigned)min(row, most) * (unsigned)(2 * a.ldk) + (ch ^ T::kx(row)) * 16;
+    constexpr int PIECES = (T::NP + NW - 1) / NW;
+    auto place = [&](bool isV, int i, int most) __attribute__((always_inline)) {
+        const int p = (wave + NW * i) * 64 + lane, row = p / nch, ch = p - row * nch;
+        return isV ? (unsigned)min(row, most) * (unsigned)(2 * a.ldv) + (ch ^ T::vx(row)) * 16
+                   : (unsigned)min(row, most) * (unsigned)(2 * a.ldk) + (ch ^ T::kx(row)) * 16;
     };
-    unsigned at[PIECES];
+    unsigned atk[PIECES], atv[PIECES];
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) at[i] = place(i, KT);
-    auto issue = [&](int t, unsigned so) __attribute__((always_inline)) {
-        const char *kt = kbase + (long)t * KT * 2 * a.ldk, *vt = vbase + (long)t * KT * 2 * a.ldv;
+    for (int i = 0; i < PIECES; ++i) atk[i] = place(false, i, KT), atv[i] = place(true, i, KT);
+    auto issue = [&](auto v_c, int t, unsigned slot) __attribute__((always_inline)) {
+        constexpr bool isV = decltype(v_c)::value;
+        const char* base = isV ? vbase + (long)t * KT * 2 * a.ldv : kbase + (long)t * KT * 2 * a.ldk;
+        const unsigned to = lds0 + (isV ? T::VOFF : 0) + slot, pitch = 1024 + (isV ? T::VGAP : T::KGAP);
         const int most = klen - 1 - key_lo - t * KT;
-        auto piece = [&](int i, unsigned from) __attribute__((always_inline)) {
-            const int idx = wave + NW * i;
-            const bool isV = idx >= npc;
-            const unsigned to = isV ? T::VOFF + (idx - npc) * (1024 + T::VGAP) : idx * (1024 + T::KGAP);
-            dma16(isV ? vt : kt, from, lds0 + so + to);
-        };
         if (most >= KT - 1) {
 #pragma unroll
             for (int i = 0; i < PIECES; ++i)
-                if (wave + NW * i < 2 * npc) piece(i, at[i]);
+                if (wave + NW * i < npc) dma16(base, isV ? atv[i] : atk[i], to + (wave + NW * i) * pitch);
         } else {
 #pragma unroll 1
-            for (int i = 0; wave + NW * i < 2 * npc; ++i) piece(i, place(i, most));
+            for (int i = 0; wave + NW * i < npc; ++i) dma16(base, place(isV, i, most), to + (wave + NW * i) * pitch);
         }
     };
-    if (nkt > 0) issue(0, 0);
+    if (nkt > 0) issue(std::false_type{}, 0, 0);
 
     bf16x8 qf[NKS];  // B operand: Q^T[16 ks + 8 hh + j][row r]
     {
@@ -265,8 +262,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
             qf[ks] = HALF ? __builtin_bit_cast(bf16x8, load_chunk_or_zero(qrow, 2 * ks + hh, nch))
                           : *reinterpret_cast<const bf16x8*>(qrow + (2 * ks + hh) * 8);
     }
-    const float slope = MOD && a.slopes ? a.slopes[gh] * LOG2E : 0.f;
-    const float c = MOD ? 1.0f : a.scale_log2;  // what a score is still multiplied by
+    const float slope = MODE & 2 ? a.slopes[gh] * LOG2E : 0.f;
+    const float c = MODE ? 1.0f : a.scale_log2;  // what a score is still multiplied by
 
     unsigned ka[T::KNX];
 #pragma unroll
@@ -303,11 +300,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
     float m = -INFINITY, lsum = 0.f;
 
-    // CUT: some row may not see all of the tile's keys
-    auto tile = [&](auto cut_c, int t, const unsigned so) __attribute__((always_inline)) {
-        constexpr bool CUT = decltype(cut_c)::value;
-        const int key0 = key_lo + t * KT;
-        f32x16 sc[KB];
+    float mc = 0.f, cf = c;  // a weight is 2^(cf score - mc)
+    f32x16 sa[KB], sb[KB];
+
+    auto qk = [&](f32x16(&sc)[KB], const unsigned so) __attribute__((always_inline)) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             f32x16 z;
@@ -315,14 +311,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
             for (int e = 0; e < 16; ++e) z[e] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks)
-            {
                 if (!GEN || 2 * ks < nch) z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfrag(so, kb, ks), qf[ks], z, 0, 0, 0);
-                if (HD > 128 && ks % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-            }
             sc[kb] = z;
         }
-        // register e of block kb scores key key0 + 32 kb + (e & 3) + 8 (e >> 2) + 4 hh
-        if (MOD && a.cap_log2 != 0.f) {  // cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)), log2(e) folded in
+    };
+    // register e of block kb scores key key0 + 32 kb + (e & 3) + 8 (e >> 2) + 4 hh; CUT: some row may not see all keys
+    auto score = [&](auto cut_c, f32x16(&sc)[KB], int t) __attribute__((always_inline)) {
+        constexpr bool CUT = decltype(cut_c)::value;
+        const int key0 = key_lo + t * KT;
+        if (MODE & 1) {  // cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)), log2(e) folded in
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -330,13 +327,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
                     const float w = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(sc[kb][e] * a.cap_in));
                     sc[kb][e] = __builtin_fmaf(-2.0f * a.cap_log2, w, a.cap_log2);
                 }
-        } else if (MOD) {
+        } else if (MODE & 2) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sc[kb][e] *= a.scale_log2;
         }
-        if (MOD && a.slopes) {
+        if (MODE & 2) {
             const float db = (float)(pq - key0 - 4 * hh);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
@@ -344,33 +341,36 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
                 for (int e = 0; e < 16; ++e)
                     sc[kb][e] = __builtin_fmaf(-slope, fabsf(db - (float)(32 * kb + (e & 3) + 8 * (e >> 2))), sc[kb][e]);
         }
-        const int lim = hi - key0 - 4 * hh;
         if (CUT) {
+            const int lim = hi - key0 - 4 * hh;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     if (32 * kb + (e & 3) + 8 * (e >> 2) >= lim) sc[kb][e] = -INFINITY;
         }
-
-        float mloc = fmaxf(sc[0][0], sc[0][1]);
+    };
+    auto largest = [&](const f32x16(&sc)[KB]) __attribute__((always_inline)) {
+        float x = fmaxf(sc[0][0], sc[0][1]);
 #pragma unroll
-        for (int e = 2; e < 16; ++e) mloc = fmaxf(mloc, sc[0][e]);
+        for (int e = 2; e < 16; ++e) x = fmaxf(x, sc[0][e]);
 #pragma unroll
         for (int kb = 1; kb < KB; ++kb)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) mloc = fmaxf(mloc, sc[kb][e]);
-        mloc = xmax32(mloc);
-        if (__builtin_amdgcn_ballot_w64((mloc - m) * c > 8.0f)) {  // P stays under 2^8 otherwise
+            for (int e = 0; e < 16; ++e) x = fmaxf(x, sc[kb][e]);
+        return xmax32(x);
+    };
+    // the running maximum takes in a tile's; O and the sum follow only where some row's grew by more than 2^8
+    auto raise = [&](float mloc, f32x16(&sc)[KB]) __attribute__((always_inline)) {
+        if (__builtin_amdgcn_ballot_w64((mloc - m) * c > 8.0f)) {
             const float mnew = fmaxf(m, mloc);
             const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mnew) * c);
             lsum *= alpha;
 #pragma unroll
             for (int i = 0; i < NDB; ++i) o[i] *= alpha;
             m = mnew;
+            mc = m == -INFINITY ? 0.f : m * c;
         }
-        const float mc = m == -INFINITY ? 0.f : m * c;
-        float cf = c;
         if (__builtin_amdgcn_ballot_w64(fabsf(mc) > 0x1p20f)) {
             // m c is rounded, s c inside the fused exponent is not: where that alone is worth whole powers of two,
             // round both
@@ -379,72 +379,92 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sc[kb][e] *= c;
             cf = 1.0f;
+        } else {
+            cf = c;
         }
-        bf16x8 pk[2 * KB];
+    };
+    auto weigh = [&](const f32x16(&sc)[KB], bf16x8(&pk)[2 * KB]) __attribute__((always_inline)) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 pk[2 * kb + (e >> 3)][e & 7] = f2bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][e], cf, -mc)));
         // the rounded weights are summed: where one weight is nearly all, its rounding divides out
-        float psum = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * KB; ++i) {
             const bf16x2 one = {1.0f, 1.0f};
-            psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 0, 1), one, psum, false);
-            psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 2, 3), one, psum, false);
-            psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 4, 5), one, psum, false);
-            psum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 6, 7), one, psum, false);
+            lsum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 0, 1), one, lsum, false);
+            lsum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 2, 3), one, lsum, false);
+            lsum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 4, 5), one, lsum, false);
+            lsum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 6, 7), one, lsum, false);
         }
-        lsum += psum;
-
+    };
+    auto pv = [&](const bf16x8(&pk)[2 * KB], const unsigned so) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 2 * KB; ++i)
 #pragma unroll
-            for (int db = 0; db < NDB; ++db) {
+            for (int db = 0; db < NDB; ++db)
                 o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfrag(so, i, db), pk[i], o[db], 0, 0, 0);
-                if (HD > 128 && db % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-            }
     };
-
     // this wave's part of the next tile has landed and its LDS reads are done; then everybody's
     auto meet = [&]() __attribute__((always_inline)) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    if (NW > 4 && wave >= NW / 2) __builtin_amdgcn_s_setprio(1);  // PRIO
+    // Tile t's weights and products beside tile t + 1's scores, which do not depend on them: the matrix pipe has work
+    // while a wave's vector instructions run. K runs one tile ahead of V, each in two slots of its own.
+    auto step = [&](auto cut_c, int t, f32x16(&s0)[KB], f32x16(&s1)[KB], const unsigned even, const unsigned odd)
+        __attribute__((always_inline)) {
+        constexpr bool CUT = decltype(cut_c)::value;
+        meet();
+        if (t + 2 < nkt) issue(std::false_type{}, t + 2, even);
+        if (t + 1 < nkt) issue(std::true_type{}, t + 1, odd);
+        bf16x8 pk[2 * KB];
+        if (!CUT || t + 1 < nkt) qk(s1, odd);
+        weigh(s0, pk);
+        pv(pk, even);
+        if (!CUT || t + 1 < nkt) {
+            score(cut_c, s1, t + 1);
+            const float mloc = largest(s1);
+            raise(mloc, s1);
+        }
+    };
+    if (NW > 4 && wave >= NW / 2) __builtin_amdgcn_s_setprio(1);
+    if (nkt > 0) {
+        meet();
+        if (nkt > 1) issue(std::false_type{}, 1, T::BYTES);
+        issue(std::true_type{}, 0, 0);
+        qk(sa, 0);
+        score(std::true_type{}, sa, 0);
+        raise(largest(sa), sa);
+    }
     int t = 0;
-    for (; t + 1 < nfull; t += 2) {  // two a turn: the ring's slots are constants
-        meet();
-        issue(t + 1, T::BYTES);
-        tile(std::false_type{}, t, 0);
-        meet();
-        if (t + 2 < nkt) issue(t + 2, 0);
-        tile(std::false_type{}, t + 1, T::BYTES);
+    for (; t + 2 < nfull; t += 2) {  // two a turn: the slots are constants
+        step(std::false_type{}, t, sa, sb, 0, T::BYTES);
+        step(std::false_type{}, t + 1, sb, sa, T::BYTES, 0);
     }
     for (; t < nkt; ++t) {
-        const unsigned so = t & 1 ? T::BYTES : 0;
-        meet();
-        if (t + 1 < nkt) issue(t + 1, T::BYTES - so);
-        if (__builtin_amdgcn_ballot_w64(hi > key_lo + t * KT)) tile(std::true_type{}, t, so);
+        const unsigned even = t & 1 ? T::BYTES : 0;
+        step(std::true_type{}, t, sa, sb, even, T::BYTES - even);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) sa[kb] = sb[kb];
     }
 
     const float l = xsum32(lsum);
     const float inv = hi > 0 ? 1.0f / l : 0.f;  // a row that sees nothing is 0
     if constexpr (SPLIT) {
         if (fr < flat) {
-            float* row = a.part + (((long)slot * a.Hkv + kvh) * a.part_rows + fr) * (a.hd + 2);
-            if (hh == 0) *reinterpret_cast<float2*>(row) = make_float2(m * c, l);
+            const long at = ((long)slot * a.Hkv + kvh) * a.part_rows + fr;
+            if (hh == 0) *reinterpret_cast<float2*>(a.stat + 2 * at) = make_float2(m * c, l);
 #pragma unroll
             for (int db = 0; db < NDB; ++db)
 #pragma unroll
                 for (int mm = 0; mm < 4; ++mm) {
                     const int d0 = 32 * db + 8 * mm + 4 * hh;
-                    if (d0 < a.hd) {
-                        *reinterpret_cast<float2*>(row + 2 + d0) = make_float2(o[db][4 * mm], o[db][4 * mm + 1]);
-                        *reinterpret_cast<float2*>(row + 4 + d0) = make_float2(o[db][4 * mm + 2], o[db][4 * mm + 3]);
-                    }
+                    if (d0 < a.hd)
+                        *reinterpret_cast<float4*>(a.part + at * a.hd + d0) =
+                            make_float4(o[db][4 * mm], o[db][4 * mm + 1], o[db][4 * mm + 2], o[db][4 * mm + 3]);
                 }
         }
     } else {
@@ -478,13 +498,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     unsigned long bad = __builtin_amdgcn_ballot_w64(fr < flat && nan != 0.f);
     bad = (bad | bad >> 32) & 0xffffffffu;
     if (bad == 0) return;
-    // keys that this wave's tiles had and some of its rows do not see: does V hold an infinity or NaN there?
+    // keys that the block's tiles had and some of this wave's rows do not see: does V hold an infinity or NaN there?
     bool found = false;
     {
-        int least = hi, most = hi;
+        int least = hi;
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) least = min(least, __shfl_xor(least, x, 64)), most = max(most, __shfl_xor(most, x, 64));
-        const int end = min(klen, key_lo + (max(most - key_lo, 0) + KT - 1) / KT * KT);
+        for (int x = 16; x > 0; x >>= 1) least = min(least, __shfl_xor(least, x, 64));
+        const int end = (int)min((long)klen, key_lo + (long)nkt * KT);
         for (int j = max(least, key_lo); j < end; ++j) {
             const bf16* v = a.v + (D.k0 + (long)j) * a.ldv + (long)kvh * a.hd;
             for (int e = lane; e < a.hd; e += 64) found |= !(fabsf(bf2f(v[e])) < INFINITY);
@@ -497,28 +517,27 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
         const int hx = min(klen, max(D.pre, px + 1));
         float mx, lx, acc[(HD + 63) / 64];
         row_alone<HD>(a, D, gx, kvh, px, qx, key_lo, SPLIT ? (int)min((long)hx, (long)key_lo + chunk) : hx, mx, lx, acc);
-        float* row = SPLIT ? a.part + (((long)slot * a.Hkv + kvh) * a.part_rows + fx) * (a.hd + 2) : nullptr;
-        if (SPLIT && lane == 0) row[0] = mx, row[1] = lx;
+        const long at = ((long)slot * a.Hkv + kvh) * a.part_rows + fx;
+        if (SPLIT && lane == 0) a.stat[2 * at] = mx, a.stat[2 * at + 1] = lx;
 #pragma unroll
         for (int cc = 0; cc < (HD + 63) / 64; ++cc) {
             const int e = lane + 64 * cc;
             if (e >= a.hd) continue;
             if (SPLIT)
-                row[2 + e] = acc[cc];
+                a.part[at * a.hd + e] = acc[cc];
             else
                 a.out[(D.q0 + (long)qx) * a.ldo + (long)gx * a.hd + e] = f2bf(hx > 0 ? acc[cc] / lx : 0.f);
         }
     }
 }
 
-// Joins a document's chunks: one wave a (document, flat row, key head), 64 columns a step.
+// Joins a document's chunks: one workgroup a (document, flat row, key head), a thread four columns of every SG-th
+// chunk, the chunks' factors 2^(m_s - max m) in LDS.
 __global__ __launch_bounds__(256) void join_docs_kernel(DocsArgs a) {
-    const int lane = threadIdx.x & 63;
-    const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int fr = (int)(w % a.part_rows);
-    const int kvh = (int)(w / a.part_rows % a.Hkv);
-    const int d = (int)(w / a.part_rows / a.Hkv);
-    if (d >= a.n) return;
+    __shared__ float wide[4], w[256], sums[4 * 256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int fr = (int)(blockIdx.x % a.part_rows), kvh = (int)(blockIdx.x / a.part_rows % a.Hkv);
+    const int d = (int)(blockIdx.x / a.part_rows / a.Hkv);
     const int q0 = clamp_row(a.qoff[d], a.rows_q), k0 = clamp_row(a.koff[d], a.rows_k);
     const int qlen = max(clamp_row(a.qoff[d + 1], a.rows_q) - q0, 0), klen = max(clamp_row(a.koff[d + 1], a.rows_k) - k0, 0);
     if (fr >= min(qlen, a.max_rows) * a.group) return;
@@ -526,31 +545,59 @@ __global__ __launch_bounds__(256) void join_docs_kernel(DocsArgs a) {
     const int pre = a.prefix ? min(max(a.prefix[d], 0), klen) : 0;
     const int hi = a.causal ? min(klen, max(pre, qi + klen - qlen + 1)) : klen;
     const int nparts = (int)(((long)klen + (1 << a.per_log2) - 1) >> a.per_log2);
-    const long step = (long)a.Hkv * a.part_rows * (a.hd + 2);
-    const float* p0 = a.part + (((long)first_slot(k0, d, 1, a.per_log2) * a.Hkv + kvh) * a.part_rows + fr) * (a.hd + 2);
+    const long row = ((long)first_slot(k0, d, 1, a.per_log2) * a.Hkv + kvh) * a.part_rows + fr;
+    const long step = (long)a.Hkv * a.part_rows;
+    const float2* stat = reinterpret_cast<const float2*>(a.stat) + row;
     float m = -INFINITY;
-    for (int s = lane; s < nparts; s += 64) m = fmaxf(m, p0[s * step]);
+    for (int s = tid; s < nparts; s += 256) m = fmaxf(m, stat[s * step].x);
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+    if (lane == 0) wide[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(wide[0], wide[1]), fmaxf(wide[2], wide[3]));
     const float mr = m == -INFINITY ? 0.f : m;
+    const int C4 = a.hd >> 2, SG = 256 / C4, col = tid % C4, sg = tid / C4;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
-    for (int s = 0; s < nparts; ++s) l = __builtin_fmaf(__builtin_amdgcn_exp2f(p0[s * step] - mr), p0[s * step + 1], l);
-    const float inv = hi > 0 ? 1.0f / l : 0.f;
-    bf16* orow = a.out + (q0 + (long)qi) * a.ldo + (long)gh * a.hd;
-    for (int col = lane; col < a.hd; col += 64) {
-        float acc = 0.f;
-        for (int s = 0; s < nparts; ++s) acc = __builtin_fmaf(__builtin_amdgcn_exp2f(p0[s * step] - mr), p0[s * step + 2 + col], acc);
-        orow[col] = f2bf(hi > 0 ? acc * inv : 0.f);
+    for (int s0 = 0; s0 < nparts; s0 += 256) {
+        const int ns = min(256, nparts - s0);
+        __syncthreads();
+        if (tid < ns) {
+            const float2 st = stat[(s0 + tid) * step];
+            w[tid] = __builtin_amdgcn_exp2f(st.x - mr);
+            l = __builtin_fmaf(w[tid], st.y, l);
+        }
+        __syncthreads();
+        if (sg < SG) {
+            const float* p = a.part + (row + s0 * step) * a.hd + 4 * col;
+#pragma unroll 4
+            for (int s = sg; s < ns; s += SG) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(p + s * step * a.hd);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(w[s], v[e], acc[e]);
+            }
+        }
+    }
+    l = wave_sum(l);
+    __syncthreads();
+    if (lane == 0) wide[wave] = l;
+    if (sg < SG) *reinterpret_cast<f32x4*>(sums + 4 * tid) = acc;  // [sg][column]
+    __syncthreads();
+    const float inv = hi > 0 ? 1.0f / ((wide[0] + wide[1]) + (wide[2] + wide[3])) : 0.f;
+    if (tid < a.hd) {
+        float o = 0.f;
+        for (int s = 0; s < SG; ++s) o += sums[s * a.hd + tid];
+        a.out[(q0 + (long)qi) * a.ldo + (long)gh * a.hd + tid] = f2bf(hi > 0 ? o * inv : 0.f);
     }
 }
 
 struct Plan {
     bool split;
     int NW, per_log2, part_rows, nslots;
-    size_t ws;
+    size_t stat, ws;
 };
 
-constexpr int NWL = 8, MINW1 = 1;
+constexpr int NWL = 8, MINW1 = 3, WANT = 2048;
 
 Plan make_plan(int n, int rows_q, int rows_k, int Hkv, int group, int hd, int max_rows) {
     Plan p{};
@@ -563,12 +610,13 @@ Plan make_plan(int n, int rows_q, int rows_k, int Hkv, int group, int hd, int ma
     if (n && mr <= 32 && rows_k / n > 256 && blocks < 2048) {
         p.split = true;
         p.NW = 1;
-        const long want = (2048 + Hkv - 1) / Hkv;  // chunks in all
-        p.per_log2 = 7;
+        const long want = (WANT + Hkv - 1) / Hkv;  // chunks in all
+        p.per_log2 = hd > 128 ? 5 : 6;  // at least a tile
         while (((long)rows_k >> p.per_log2) > want) ++p.per_log2;
         p.part_rows = (int)mr;
         nslots = ((long)rows_k >> p.per_log2) + n;
-        p.ws = (size_t)nslots * Hkv * mr * (hd + 2) * 4;
+        p.stat = (size_t)nslots * Hkv * mr * hd;  // where the statistics begin, in floats
+        p.ws = (p.stat + (size_t)nslots * Hkv * mr * 2) * 4;
     }
     p.nslots = nslots * Hkv < (1L << 31) ? (int)nslots : -1;
     return p;
@@ -577,10 +625,12 @@ Plan make_plan(int n, int rows_q, int rows_k, int Hkv, int group, int hd, int ma
 template <int HD, bool GEN, int NW, int MINW, bool SPLIT>
 void launch_docs(const DocsArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)(a.nslots * a.Hkv)), block(NW * 64);
-    if (a.cap_log2 != 0.f || a.slopes)
-        hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, SPLIT, true>), grid, block, 0, s, a);
-    else
-        hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, SPLIT, false>), grid, block, 0, s, a);
+    switch ((a.cap_log2 != 0.f ? 1 : 0) | (a.slopes ? 2 : 0)) {
+        case 0: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, SPLIT, 0>), grid, block, 0, s, a); break;
+        case 1: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, SPLIT, 1>), grid, block, 0, s, a); break;
+        case 2: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, SPLIT, 2>), grid, block, 0, s, a); break;
+        default: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, SPLIT, 3>), grid, block, 0, s, a);
+    }
 }
 
 template <int HD, bool GEN, int MINW>
@@ -629,13 +679,13 @@ extern "C" int mme_attention_docs(const void* q, long ldq, const void* k, long l
     const int mr = max_rows < rows_q ? max_rows : rows_q;
     if (mr == 0) return MME_OK;
     const Plan p = make_plan(n, rows_q, rows_k, Hkv, Hq / Hkv, hd, mr);
-    MME_REQUIRE(p.nslots >= 0 && (long)rows_q * (Hq / Hkv) < (1L << 31) - 512 && (long)n * Hkv * p.part_rows < (1L << 33),
+    MME_REQUIRE(p.nslots >= 0 && (long)rows_q * (Hq / Hkv) < (1L << 31) - 512 && (long)n * Hkv * p.part_rows < (1L << 31),
                 "mme_attention_docs: too many rows");
     MME_REQUIRE(p.ws == 0 || (workspace && ws_bytes >= p.ws && ((uintptr_t)workspace & 15) == 0),
                 "mme_attention_docs: workspace of %zu bytes, %zu needed", ws_bytes, p.ws);
     DocsArgs a{};
     a.q = (const bf16*)q, a.k = (const bf16*)k, a.v = (const bf16*)v, a.out = (bf16*)out;
-    a.qoff = q_offsets, a.koff = k_offsets, a.prefix = prefix, a.slopes = slopes, a.part = (float*)workspace;
+    a.qoff = q_offsets, a.koff = k_offsets, a.prefix = prefix, a.slopes = slopes, a.part = (float*)workspace, a.stat = a.part + p.stat;
     a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldo = ldo, a.nslots = p.nslots;
     a.n = n, a.rows_q = rows_q, a.rows_k = rows_k, a.Hkv = Hkv, a.group = Hq / Hkv, a.hd = hd;
     a.max_rows = mr, a.causal = causal ? 1 : 0, a.per_log2 = p.per_log2, a.part_rows = p.part_rows;
@@ -659,7 +709,7 @@ extern "C" int mme_attention_docs(const void* q, long ldq, const void* k, long l
     }
     if (p.split) {
         if (int rc = mme_check_launch("mme_attention_docs")) return rc;
-        hipLaunchKernelGGL(join_docs_kernel, dim3((unsigned)cdiv((long)n * Hkv * p.part_rows, 4)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(join_docs_kernel, dim3((unsigned)((long)n * Hkv * p.part_rows)), dim3(256), 0, s, a);
     }
     return mme_check_launch("mme_attention_docs");
 }

@@ -450,12 +450,24 @@ def attention_mqa(qkv: torch.Tensor, B: int, T: int, Hq: int, hd: int, *, kstart
 
 
 # ---------------------------------------------------------------- packed documents
-def _on_device_of(t: torch.Tensor, *ts: Optional[torch.Tensor]):
-    """A context in which t's device is the current one (so its stream is taken); all tensors lie there."""
+_raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index; torch.cuda.current_stream() takes 2.6 us more
+
+
+def _one_device(name: str, t: torch.Tensor, *ts: Optional[torch.Tensor]) -> int:
+    """The index of the one device that all tensors lie on."""
+    dev = t.get_device()
+    if dev < 0:
+        _dev(t)
     for u in ts:
-        if u is not None and u.device != t.device:
-            raise ValueError(f"tensors on two devices: {t.device} and {u.device}")
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+        if u is not None and u.get_device() != dev:
+            _dev(u)
+            raise ValueError(f"{name}: tensors on two devices: {t.device} and {u.device}")
+    return dev
+
+
+def _on(dev: int):
+    """A context in which device dev is the current one."""
+    return torch.cuda.device(dev)
 
 
 def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axes: torch.Tensor, nheads: int, *,
@@ -469,29 +481,35 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axe
     or (2i, 2i + 1) with adjacent; elements from 2 * pairs on are copied. inverse turns back: the gradient with
     respect to x is this of the gradient with respect to the result. out: None for a new tensor, x itself for in
     place, or one that does not overlap x."""
-    _dev(x, positions, freqs, axes, out)
+    dev = _one_device("rope_axes", x, positions, freqs, axes, out)
+    if dev != torch.cuda.current_device():
+        with _on(dev):
+            return rope_axes(x, positions, freqs, axes, nheads, hd=hd, adjacent=adjacent, inverse=inverse, out=out)
     ldx = _rowmajor(x, "x")
-    rows, pairs = x.shape[0], freqs.numel()
-    hd = x.shape[1] // max(nheads, 1) if hd is None else hd
-    if x.dtype != BF16 or (out is not None and out.dtype != BF16):
-        raise ValueError("rope_axes: x and out must be bf16")
-    if nheads < 1 or pairs < 1 or 2 * pairs > hd or nheads * hd > x.shape[1]:
-        raise ValueError(f"rope_axes: {nheads} heads of {hd} with {pairs} pairs do not fit rows of {x.shape[1]}")
-    if positions.dtype != torch.int32 or positions.dim() != 2 or positions.shape[1] != rows or positions.shape[0] < 1 \
-            or (rows > 1 and positions.stride(1) != 1):
+    (rows, width), pairs = x.shape, freqs.numel()
+    hd = width // max(nheads, 1) if hd is None else hd
+    if x.dtype is not BF16:
+        raise ValueError("rope_axes: x must be bf16")
+    if nheads < 1 or pairs < 1 or 2 * pairs > hd or nheads * hd > width:
+        raise ValueError(f"rope_axes: {nheads} heads of {hd} with {pairs} pairs do not fit rows of {width}")
+    if positions.dtype is not torch.int32 or positions.dim() != 2 or positions.shape[1] != rows \
+            or positions.shape[0] < 1 or (rows > 1 and positions.stride(1) != 1):
         raise ValueError(f"rope_axes: positions must be int32 [axes, {rows}] with contiguous rows")
-    if freqs.dtype != torch.float64 or axes.dtype != torch.int32 or axes.numel() != pairs or freqs.dim() != 1 \
+    if freqs.dtype is not torch.float64 or axes.dtype is not torch.int32 or axes.numel() != pairs or freqs.dim() != 1 \
             or not (freqs.is_contiguous() and axes.is_contiguous()):
         raise ValueError("rope_axes: freqs must be contiguous float64 [pairs] and axes int32 [pairs]")
-    with _on_device_of(x, positions, freqs, axes, out):
-        if out is None:
-            out = torch.empty(rows, nheads * hd, dtype=BF16, device=x.device)
-        elif out.dim() != 2 or out.shape[0] != rows or out.shape[1] < nheads * hd:
-            raise ValueError(f"rope_axes: out must be [{rows}, >= {nheads * hd}]")
-        ev = KernelTimer.begin()
-        call("mme_rope_axes", x.data_ptr(), ldx, out.data_ptr(), _rowmajor(out, "out"), rows, nheads, hd, pairs,
-             positions.data_ptr(), max(positions.stride(0), rows), positions.shape[0], freqs.data_ptr(),
-             axes.data_ptr(), int(adjacent), int(inverse), _stream())
+    if out is None:
+        out = torch.empty(rows, nheads * hd, dtype=BF16, device=x.device)
+        ldo = nheads * hd
+    elif out.dtype is not BF16 or out.dim() != 2 or out.shape[0] != rows or out.shape[1] < nheads * hd:
+        raise ValueError(f"rope_axes: out must be bf16 [{rows}, >= {nheads * hd}]")
+    else:
+        ldo = _rowmajor(out, "out")
+    ev = KernelTimer.begin()
+    call("mme_rope_axes", x.data_ptr(), ldx, out.data_ptr(), ldo, rows, nheads, hd, pairs, positions.data_ptr(),
+         max(positions.stride(0), rows), positions.shape[0], freqs.data_ptr(), axes.data_ptr(), adjacent, inverse,
+         _raw_stream(dev))
+    if ev is not None:
         KernelTimer.end(ev, "rope_axes", 0.0, 4.0 * rows * nheads * hd)
     return out
 
@@ -532,40 +550,49 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: t
     query a document: max_rows=1), so that the keys are split over the device. Rows of no document, and a document's
     rows from max_rows on, are left as they were (not set in a new out)."""
     key_offsets = offsets if key_offsets is None else key_offsets
-    _dev(q, k, v, offsets, key_offsets, prefix, slopes, out)
+    dev = _one_device("attention_docs", q, k, v, offsets, key_offsets, prefix, slopes, out)
+    if dev != torch.cuda.current_device():
+        with _on(dev):
+            return attention_docs(q, k, v, offsets, heads, kv_heads, key_offsets=key_offsets, max_rows=max_rows,
+                                  causal=causal, prefix=prefix, softcap=softcap, slopes=slopes, scale=scale, out=out)
     ldq, ldk, ldv = _rowmajor(q, "q"), _rowmajor(k, "k"), _rowmajor(v, "v")
-    if heads < 1 or kv_heads < 1 or heads % kv_heads or q.shape[1] % heads:
-        raise ValueError(f"attention_docs: {heads} heads over {kv_heads} key heads in rows of {q.shape[1]}")
-    hd, rows, keys, n = q.shape[1] // heads, q.shape[0], k.shape[0], offsets.numel() - 1
-    if any(t.dtype != BF16 for t in (q, k, v)) or (out is not None and out.dtype != BF16):
-        raise ValueError("attention_docs: q, k, v and out must be bf16")
+    (rows, width), keys, n = q.shape, k.shape[0], offsets.numel() - 1
+    if heads < 1 or kv_heads < 1 or heads % kv_heads or width % heads:
+        raise ValueError(f"attention_docs: {heads} heads over {kv_heads} key heads in rows of {width}")
+    hd = width // heads
+    if q.dtype is not BF16 or k.dtype is not BF16 or v.dtype is not BF16:
+        raise ValueError("attention_docs: q, k and v must be bf16")
     if k.shape != v.shape or k.shape[1] != kv_heads * hd:
         raise ValueError(f"attention_docs: k {tuple(k.shape)} and v {tuple(v.shape)} must be [keys, {kv_heads * hd}]")
-    if n < 0 or key_offsets.numel() != n + 1 or any(
-            t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() for t in (offsets, key_offsets)):
-        raise ValueError("attention_docs: offsets and key_offsets must be contiguous int32 [documents + 1]")
-    if prefix is not None and (prefix.dtype != torch.int32 or prefix.numel() != n or not prefix.is_contiguous()):
-        raise ValueError("attention_docs: prefix must be contiguous int32 [documents]")
-    if prefix is not None and not causal:
-        raise ValueError("attention_docs: a prefix goes with the causal mask")
-    if slopes is not None and (slopes.dtype != torch.float32 or slopes.numel() != heads or not slopes.is_contiguous()):
+    for t in (offsets, key_offsets):
+        if n < 0 or t.numel() != n + 1 or t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            raise ValueError("attention_docs: offsets and key_offsets must be contiguous int32 [documents + 1]")
+    if prefix is not None:
+        if prefix.dtype is not torch.int32 or prefix.numel() != n or not prefix.is_contiguous():
+            raise ValueError("attention_docs: prefix must be contiguous int32 [documents]")
+        if not causal:
+            raise ValueError("attention_docs: a prefix goes with the causal mask")
+    if slopes is not None and (slopes.dtype is not torch.float32 or slopes.numel() != heads
+                               or not slopes.is_contiguous()):
         raise ValueError("attention_docs: slopes must be contiguous fp32 [heads]")
     if max_rows is not None and max_rows < 0:
         raise ValueError("attention_docs: max_rows must not be negative")
     max_rows = rows if max_rows is None else min(int(max_rows), rows)
-    scale = hd ** -0.5 if scale is None else scale
-    with _on_device_of(q, k, v, offsets, key_offsets, prefix, slopes, out):
-        if out is None:
-            out = torch.empty(rows, heads * hd, dtype=BF16, device=q.device)
-        elif out.dim() != 2 or out.shape[0] != rows or out.shape[1] < heads * hd:
-            raise ValueError(f"attention_docs: out must be [{rows}, >= {heads * hd}]")
-        wsb = query("mme_attention_docs_workspace_bytes", n, rows, keys, heads, kv_heads, hd, max_rows)
-        # a workspace of the call's own: calls on two streams, or in two captured graphs, share none
-        ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
-        ev = KernelTimer.begin()
-        call("mme_attention_docs", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(),
-             _rowmajor(out, "out"), offsets.data_ptr(), key_offsets.data_ptr(), n, rows, keys, heads, kv_heads, hd,
-             max_rows, int(causal), _ptr(prefix), float(softcap), _ptr(slopes), float(scale), _ptr(ws), wsb, _stream())
+    if out is None:
+        out = torch.empty(rows, width, dtype=BF16, device=q.device)
+        ldo = width
+    elif out.dtype is not BF16 or out.dim() != 2 or out.shape[0] != rows or out.shape[1] < width:
+        raise ValueError(f"attention_docs: out must be bf16 [{rows}, >= {width}]")
+    else:
+        ldo = _rowmajor(out, "out")
+    wsb = query("mme_attention_docs_workspace_bytes", n, rows, keys, heads, kv_heads, hd, max_rows)
+    # a workspace of the call's own: calls on two streams, or in two captured graphs, share none
+    ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
+    ev = KernelTimer.begin()
+    call("mme_attention_docs", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo,
+         offsets.data_ptr(), key_offsets.data_ptr(), n, rows, keys, heads, kv_heads, hd, max_rows, bool(causal),
+         _ptr(prefix), softcap, _ptr(slopes), hd ** -0.5 if scale is None else scale, _ptr(ws), wsb, _raw_stream(dev))
+    if ev is not None:
         # which pairs are visible is on the device: the bytes alone are known here
         KernelTimer.end(ev, "attention_docs", 0.0, 4.0 * rows * heads * hd + 4.0 * keys * kv_heads * hd)
     return out
