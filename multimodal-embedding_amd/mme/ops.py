@@ -453,21 +453,12 @@ def attention_mqa(qkv: torch.Tensor, B: int, T: int, Hq: int, hd: int, *, kstart
 _raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index; torch.cuda.current_stream() takes 2.6 us more
 
 
-def _one_device(name: str, t: torch.Tensor, *ts: Optional[torch.Tensor]) -> int:
-    """The index of the one device that all tensors lie on."""
-    dev = t.get_device()
-    if dev < 0:
-        _dev(t)
+def _elsewhere(name: str, t: torch.Tensor, *ts: Optional[torch.Tensor]) -> None:
+    """Raises if the tensors do not lie on one device."""
+    _dev(t, *ts)
     for u in ts:
-        if u is not None and u.get_device() != dev:
-            _dev(u)
+        if u is not None and u.device != t.device:
             raise ValueError(f"{name}: tensors on two devices: {t.device} and {u.device}")
-    return dev
-
-
-def _on(dev: int):
-    """A context in which device dev is the current one."""
-    return torch.cuda.device(dev)
 
 
 def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axes: torch.Tensor, nheads: int, *,
@@ -481,9 +472,12 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axe
     or (2i, 2i + 1) with adjacent; elements from 2 * pairs on are copied. inverse turns back: the gradient with
     respect to x is this of the gradient with respect to the result. out: None for a new tensor, x itself for in
     place, or one that does not overlap x."""
-    dev = _one_device("rope_axes", x, positions, freqs, axes, out)
+    dev = x.get_device()
+    if dev < 0 or not dev == positions.get_device() == freqs.get_device() == axes.get_device() \
+            or (out is not None and out.get_device() != dev):
+        _elsewhere("rope_axes", x, positions, freqs, axes, out)
     if dev != torch.cuda.current_device():
-        with _on(dev):
+        with torch.cuda.device(dev):
             return rope_axes(x, positions, freqs, axes, nheads, hd=hd, adjacent=adjacent, inverse=inverse, out=out)
     ldx = _rowmajor(x, "x")
     (rows, width), pairs = x.shape, freqs.numel()
@@ -492,11 +486,13 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axe
         raise ValueError("rope_axes: x must be bf16")
     if nheads < 1 or pairs < 1 or 2 * pairs > hd or nheads * hd > width:
         raise ValueError(f"rope_axes: {nheads} heads of {hd} with {pairs} pairs do not fit rows of {width}")
-    if positions.dtype is not torch.int32 or positions.dim() != 2 or positions.shape[1] != rows \
-            or positions.shape[0] < 1 or (rows > 1 and positions.stride(1) != 1):
+    if positions.dim() != 2 or positions.dtype is not torch.int32:
+        raise ValueError(f"rope_axes: positions must be int32 [axes, {rows}]")
+    (naxes, cols), (ldp, step) = positions.shape, positions.stride()
+    if cols != rows or naxes < 1 or (rows > 1 and step != 1):
         raise ValueError(f"rope_axes: positions must be int32 [axes, {rows}] with contiguous rows")
-    if freqs.dtype is not torch.float64 or axes.dtype is not torch.int32 or axes.numel() != pairs or freqs.dim() != 1 \
-            or not (freqs.is_contiguous() and axes.is_contiguous()):
+    if freqs.dtype is not torch.float64 or axes.dtype is not torch.int32 or axes.shape != freqs.shape \
+            or freqs.dim() != 1 or not (freqs.is_contiguous() and axes.is_contiguous()):
         raise ValueError("rope_axes: freqs must be contiguous float64 [pairs] and axes int32 [pairs]")
     if out is None:
         out = torch.empty(rows, nheads * hd, dtype=BF16, device=x.device)
@@ -507,8 +503,7 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axe
         ldo = _rowmajor(out, "out")
     ev = KernelTimer.begin()
     call("mme_rope_axes", x.data_ptr(), ldx, out.data_ptr(), ldo, rows, nheads, hd, pairs, positions.data_ptr(),
-         max(positions.stride(0), rows), positions.shape[0], freqs.data_ptr(), axes.data_ptr(), adjacent, inverse,
-         _raw_stream(dev))
+         ldp if ldp > rows else rows, naxes, freqs.data_ptr(), axes.data_ptr(), adjacent, inverse, _raw_stream(dev))
     if ev is not None:
         KernelTimer.end(ev, "rope_axes", 0.0, 4.0 * rows * nheads * hd)
     return out
@@ -550,9 +545,12 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: t
     query a document: max_rows=1), so that the keys are split over the device. Rows of no document, and a document's
     rows from max_rows on, are left as they were (not set in a new out)."""
     key_offsets = offsets if key_offsets is None else key_offsets
-    dev = _one_device("attention_docs", q, k, v, offsets, key_offsets, prefix, slopes, out)
+    dev = q.get_device()
+    if dev < 0 or not dev == k.get_device() == v.get_device() == offsets.get_device() == key_offsets.get_device() \
+            or any(t is not None and t.get_device() != dev for t in (prefix, slopes, out)):
+        _elsewhere("attention_docs", q, k, v, offsets, key_offsets, prefix, slopes, out)
     if dev != torch.cuda.current_device():
-        with _on(dev):
+        with torch.cuda.device(dev):
             return attention_docs(q, k, v, offsets, heads, kv_heads, key_offsets=key_offsets, max_rows=max_rows,
                                   causal=causal, prefix=prefix, softcap=softcap, slopes=slopes, scale=scale, out=out)
     ldq, ldk, ldv = _rowmajor(q, "q"), _rowmajor(k, "k"), _rowmajor(v, "v")
@@ -564,7 +562,7 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: t
         raise ValueError("attention_docs: q, k and v must be bf16")
     if k.shape != v.shape or k.shape[1] != kv_heads * hd:
         raise ValueError(f"attention_docs: k {tuple(k.shape)} and v {tuple(v.shape)} must be [keys, {kv_heads * hd}]")
-    for t in (offsets, key_offsets):
+    for t in (offsets,) if key_offsets is offsets else (offsets, key_offsets):
         if n < 0 or t.numel() != n + 1 or t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
             raise ValueError("attention_docs: offsets and key_offsets must be contiguous int32 [documents + 1]")
     if prefix is not None:
