@@ -42,6 +42,7 @@ struct DocsArgs {
     float *part, *stat;  // split: O [slot][key head][flat row][hd], and (maximum, sum) [slot][key head][flat row][2]
     long ldq, ldk, ldv, ldo;
     int nslots, n, rows_q, rows_k, Hkv, group, hd, max_rows, causal, part_rows;
+    int sorted;
     int per_log2;       // a slot's flat rows, or keys (split), are 1 << per_log2
     float scale_log2, cap_log2, cap_in;
 };
@@ -69,7 +70,9 @@ __device__ __forceinline__ int first_slot(int off, int d, int mul, int sh) { ret
 struct Doc {
     int d, q0, qlen, k0, klen, pre, first;
 };
-template <bool SPLIT>
+// SORT: with at most 63 documents and many workgroups (a.sorted) the slots go by documents, the one with most keys
+// first, so that no long document is begun when the others are done.
+template <bool SPLIT, bool SORT>
 __device__ __forceinline__ Doc find_doc(const DocsArgs& a, int slot) {
     const int lane = threadIdx.x & 63;
     const int32_t* off = SPLIT ? a.koff : a.qoff;
@@ -89,15 +92,27 @@ __device__ __forceinline__ Doc find_doc(const DocsArgs& a, int slot) {
     const int i = min(lo + lane, a.n);
     const int qo = clamp_row(a.qoff[i], a.rows_q), ko = clamp_row(a.koff[i], a.rows_k);
     const int pr = a.prefix ? a.prefix[min(i, a.n - 1)] : 0;
-    const int fs = first_slot(SPLIT ? ko : qo, i, mul, a.per_log2);
-    const int c = __popcll(__builtin_amdgcn_ballot_w64(lo + lane < hi && fs <= slot));
-    const int l = c > 0 ? c - 1 : 0;
+    int fs = first_slot(SPLIT ? ko : qo, i, mul, a.per_log2), l;
+    if (SORT && a.sorted) {
+        const int kl = lane < a.n ? __shfl_down(ko, 1, 64) - ko : -1;
+        const int parts = lane < a.n ? (min(max(__shfl_down(qo, 1, 64) - qo, 0), a.max_rows) * mul + (1 << a.per_log2) - 1) >> a.per_log2 : 0;
+        fs = 0;  // the slots of the documents before this lane's
+        for (int j = 0; j < a.n; ++j) {
+            const int kj = __builtin_amdgcn_readlane(kl, j), pj = __builtin_amdgcn_readlane(parts, j);
+            fs += kj > kl || (kj == kl && j < lane) ? pj : 0;
+        }
+        const unsigned long at = __builtin_amdgcn_ballot_w64(fs <= slot && slot < fs + parts);
+        l = at ? __builtin_ctzll(at) : 63;  // none: the last lane, whose document has no rows
+    } else {
+        const int c = __popcll(__builtin_amdgcn_ballot_w64(lo + lane < hi && fs <= slot));
+        l = c > 0 ? c - 1 : 0;
+    }
     Doc r;
     r.d = lo + l;
     r.q0 = __builtin_amdgcn_readlane(qo, l);
     r.k0 = __builtin_amdgcn_readlane(ko, l);
-    r.qlen = max(__builtin_amdgcn_readlane(qo, l + 1) - r.q0, 0);
-    r.klen = max(__builtin_amdgcn_readlane(ko, l + 1) - r.k0, 0);
+    r.qlen = max(__builtin_amdgcn_readlane(qo, min(l + 1, 63)) - r.q0, 0);
+    r.klen = max(__builtin_amdgcn_readlane(ko, min(l + 1, 63)) - r.k0, 0);
     r.pre = min(max(__builtin_amdgcn_readlane(pr, l), 0), r.klen);
     r.first = __builtin_amdgcn_readlane(fs, l);
     return r;
@@ -120,9 +135,14 @@ struct Tile {
     static constexpr int KGAP = XOR ? 16 : 0, VGAP = XOR && HD == 256 ? 64 : 0;
     static __device__ __forceinline__ int kx(int row) { return !XOR ? 0 : KX * ((HD == 64 ? row >> 1 : row) & (KNX - 1)); }
     static __device__ __forceinline__ int vx(int row) { return !XOR ? 0 : VX * ((HD == 64 ? row >> 1 : row) & (VNX - 1)); }
-    static constexpr int NP = KT * HD / 512;           // pieces of K, and of V
-    static constexpr int VOFF = NP * (1024 + KGAP);
-    static constexpr int BYTES = VOFF + NP * (1024 + VGAP) + (HD % 32 ? 64 : 0);  // the last block reads past a row
+    // Head dims 72 and 80 leave columns of O^T free: V's rows in LDS have 12 chunks, which the copies fill up to the head
+    // dim; the next holds ones, which sums the weights. 12 chunks put the 4 rows of a transposed read, and an odd number
+    // the 16 rows of a K read, into banks of their own.
+    static constexpr bool ONES = HD == 72 || HD == 80;
+    static constexpr int KP = ONES ? 9 + (HD == 80 ? 2 : 0) : HD / 8, VP = ONES ? 12 : HD / 8;  // chunks a row (not GEN)
+    static constexpr int NPK = KT * KP / 64, NPV = KT * VP / 64;                                // pieces of K, and of V
+    static constexpr int VOFF = NPK * (1024 + KGAP);
+    static constexpr int BYTES = VOFF + NPV * (1024 + VGAP);
     // where row `row` of K or V begins (rows of a piece are contiguous); nch: chunks a row
     static __device__ __forceinline__ int at(int row, int nch, int gap) {
         return row * nch * 16 + (XOR ? row / (512 / HD) * gap : 0);
@@ -174,27 +194,35 @@ __device__ __forceinline__ void row_alone(const DocsArgs& a, const Doc& D, int g
 }
 
 // MODE: 1 = capped scores, 2 = biased by distance, 3 = both
-template <int HD, bool GEN, int NW, int MINW, bool SPLIT, int MODE>
+// AHEAD: the next tile's scores are formed beside this one's weights; NS: slots of the ring
+template <int HD, bool GEN, int NW, int MINW, int NS, bool AHEAD, bool SPLIT, int MODE>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW))) void attn_docs_kernel(DocsArgs a) {
     using T = Tile<HD, GEN>;
     constexpr int KT = T::KT, KB = T::KB, NKS = T::NKS, NDB = T::NDB, QB = NW * 32;
     constexpr bool HALF = GEN || HD % 16 != 0;  // the last k-step may reach past the head dim
-    constexpr int ZERO = 2 * T::BYTES;           // 16 zero bytes for it
-    __shared__ __attribute__((aligned(16))) char lds[2 * T::BYTES + (HALF ? 16 : 0)];
+    constexpr int ZERO = NS * T::BYTES;           // 16 zero bytes for it
+    __shared__ __attribute__((aligned(16))) char lds[NS * T::BYTES + (HALF ? 16 : 0)];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, hh = lane >> 5;
-    int id;
-    {  // consecutive work on one XCD: slots of one key head (the same K / V)
+    // Workgroups go round the 8 XCDs. Where the K / V of a slot are its own, the key heads go side by side, as their
+    // rows lie in shared lines; else an XCD keeps to as few key heads as it can, whose K / V its slots share, and takes
+    // their slots side by side, so that all heads' first slots (the longest, where they are sorted) start first.
+    constexpr bool OWN = SPLIT || NW == 1;
+    int slot, kvh;
+    {
         const int bid = blockIdx.x, nwg = gridDim.x;
         const int xcd = bid & 7, loc = bid >> 3, q8 = nwg >> 3, r8 = nwg & 7;
-        id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + loc;
+        const int id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + loc;
+        if (OWN)
+            slot = id / a.Hkv, kvh = id - slot * a.Hkv;
+        else if ((a.Hkv & 7) == 0)
+            slot = loc / (a.Hkv >> 3), kvh = xcd * (a.Hkv >> 3) + loc - slot * (a.Hkv >> 3);
+        else
+            kvh = id / a.nslots, slot = id - kvh * a.nslots;
     }
-    // where the K / V of a slot are its own, the key heads go side by side, as their rows lie in shared lines
-    constexpr bool OWN = SPLIT || NW == 1;
-    const int slot = OWN ? id / a.Hkv : id % a.nslots, kvh = OWN ? id % a.Hkv : id / a.nslots;
-    const Doc D = find_doc<SPLIT>(a, slot);
+    const Doc D = find_doc<SPLIT, !OWN>(a, slot);
     const int qlen = D.qlen, klen = D.klen;
     const int flat = min(qlen, a.max_rows) * a.group;  // flat rows of this document
     int part = slot - D.first;
@@ -220,36 +248,49 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     const int nfull = (hi_min - key_lo) / KT;  // tiles that every row sees whole (none where negative)
     const int nkt = hi_max > key_lo ? (hi_max - key_lo + KT - 1) / KT : 0;
 
-    const int nch = GEN ? a.hd >> 3 : HD / 8;  // 16-byte chunks a row, in memory and in LDS
+    const int nch = GEN ? a.hd >> 3 : HD / 8;                               // 16-byte chunks of a row
+    const int kp = GEN ? nch : T::KP, vp = GEN ? nch : T::VP;               // and between rows in LDS
     if (HALF && tid == 0) *reinterpret_cast<u16x8*>(lds + ZERO) = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
 
     const unsigned lds0 = (unsigned)(uintptr_t)(LDS_AS char*)lds;
     const char* kbase = (const char*)(a.k + (D.k0 + (long)key_lo) * a.ldk + (long)kvh * a.hd);
     const char* vbase = (const char*)(a.v + (D.k0 + (long)key_lo) * a.ldv + (long)kvh * a.hd);
-    // a tile of K (or V) is nch * KT / 64 pieces; piece p: LDS chunks 64 p .. + 63, chunk c of row (64 p + lane) / nch.
+    // a tile of K (V) is kp (vp) * KT / 64 pieces; piece p: LDS chunks 64 p .. + 63, chunk c of row (64 p + lane) / kp.
     // A lane's places in them are the same in every tile but one that reaches past the document.
-    const int npc = nch * KT / 64;
-    constexpr int PIECES = (T::NP + NW - 1) / NW;
+    const int npk = GEN ? nch * KT / 64 : T::NPK, npv = GEN ? nch * KT / 64 : T::NPV;
+    if (T::ONES)
+        for (int i = tid; i < NS * KT; i += NW * 64)
+            *reinterpret_cast<u16x8*>(lds + i / KT * T::BYTES + T::VOFF + (i % KT * T::VP + HD / 8) * 16) =
+                u16x8{0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80};
+    auto row_of = [&](bool isV, int i) __attribute__((always_inline)) { return ((wave + NW * i) * 64 + lane) / (isV ? vp : kp); };
+    auto chunk_of = [&](bool isV, int i) __attribute__((always_inline)) { return ((wave + NW * i) * 64 + lane) % (isV ? vp : kp); };
     auto place = [&](bool isV, int i, int most) __attribute__((always_inline)) {
-        const int p = (wave + NW * i) * 64 + lane, row = p / nch, ch = p - row * nch;
+        const int row = row_of(isV, i), ch = chunk_of(isV, i);
         return isV ? (unsigned)min(row, most) * (unsigned)(2 * a.ldv) + (ch ^ T::vx(row)) * 16
                    : (unsigned)min(row, most) * (unsigned)(2 * a.ldk) + (ch ^ T::kx(row)) * 16;
     };
-    unsigned atk[PIECES], atv[PIECES];
+    constexpr int PK = (T::NPK + NW - 1) / NW, PV = (T::NPV + NW - 1) / NW;
+    constexpr bool KFULL = GEN || T::KP == HD / 8, VFULL = GEN || T::VP == HD / 8;  // no chunk to leave out
+    unsigned atk[PK], atv[PV];
+    bool dok[PK], dov[PV];
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) atk[i] = place(false, i, KT), atv[i] = place(true, i, KT);
+    for (int i = 0; i < PK; ++i) atk[i] = place(false, i, KT), dok[i] = chunk_of(false, i) < nch;
+#pragma unroll
+    for (int i = 0; i < PV; ++i) atv[i] = place(true, i, KT), dov[i] = chunk_of(true, i) < nch;
     auto issue = [&](auto v_c, int t, unsigned slot) __attribute__((always_inline)) {
         constexpr bool isV = decltype(v_c)::value;
         const char* base = isV ? vbase + (long)t * KT * 2 * a.ldv : kbase + (long)t * KT * 2 * a.ldk;
         const unsigned to = lds0 + (isV ? T::VOFF : 0) + slot, pitch = 1024 + (isV ? T::VGAP : T::KGAP);
-        const int most = klen - 1 - key_lo - t * KT;
+        const int most = klen - 1 - key_lo - t * KT, np = isV ? npv : npk;
         if (most >= KT - 1) {
 #pragma unroll
-            for (int i = 0; i < PIECES; ++i)
-                if (wave + NW * i < npc) dma16(base, isV ? atv[i] : atk[i], to + (wave + NW * i) * pitch);
+            for (int i = 0; i < (isV ? PV : PK); ++i)
+                if (wave + NW * i < np && ((isV ? VFULL : KFULL) || (isV ? dov[i] : dok[i])))
+                    dma16(base, isV ? atv[i] : atk[i], to + (wave + NW * i) * pitch);
         } else {
 #pragma unroll 1
-            for (int i = 0; wave + NW * i < npc; ++i) dma16(base, place(isV, i, most), to + (wave + NW * i) * pitch);
+            for (int i = 0; wave + NW * i < np; ++i)
+                if ((isV ? VFULL : KFULL) || chunk_of(isV, i) < nch) dma16(base, place(isV, i, most), to + (wave + NW * i) * pitch);
         }
     };
     if (nkt > 0) issue(std::false_type{}, 0, 0);
@@ -267,11 +308,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
 
     unsigned ka[T::KNX];
 #pragma unroll
-    for (int g = 0; g < T::KNX; ++g) ka[g] = lds0 + T::at(r, nch, T::KGAP) + (((g * T::KX) ^ T::kx(r)) + hh) * 16;
+    for (int g = 0; g < T::KNX; ++g) ka[g] = lds0 + T::at(r, kp, T::KGAP) + (((g * T::KX) ^ T::kx(r)) + hh) * 16;
     auto kfrag = [&](unsigned so, int kb, int ks) __attribute__((always_inline)) {
         constexpr int U = T::KX / 2, W = T::KNX * U;  // k-steps a unit, and all units
         unsigned at = (T::XOR ? ka[ks / U % T::KNX] + (ks % U + ks / W * W) * 32 : ka[0] + ks * 32) + so +
-                      kb * T::at(32, nch, T::KGAP);
+                      kb * T::at(32, kp, T::KGAP);
         if (HALF && (GEN || ks == NKS - 1)) at = 2 * ks + hh < nch ? at : lds0 + ZERO;
         return *reinterpret_cast<const LDS_AS bf16x8*>((uintptr_t)at);
     };
@@ -281,15 +322,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
         const int i16 = lane & 15, q = i16 >> 2, p = i16 & 3, half = (lane >> 4) & 1;
 #pragma unroll
         for (int g = 0; g < T::VNX; ++g)
-            va[g] = lds0 + T::VOFF + T::at(4 * hh + q, nch, T::VGAP) + (((g * T::VX) ^ T::vx(q)) + 2 * half + (p >> 1)) * 16 +
+            va[g] = lds0 + T::VOFF + T::at(4 * hh + q, vp, T::VGAP) + (((g * T::VX) ^ T::vx(q)) + 2 * half + (p >> 1)) * 16 +
                     (p & 1) * 8;
     }
     auto vfrag = [&](unsigned so, int i, int db) __attribute__((always_inline)) {
         constexpr int U = T::VX / 4, W = T::VNX * U;
         const unsigned at = (T::XOR ? va[db / U % T::VNX] + (db % U + db / W * W) * 64 : va[0] + db * 64) + so +
-                            i * T::at(16, nch, T::VGAP);
+                            i * T::at(16, vp, T::VGAP);
         const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(uintptr_t)at);
-        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(uintptr_t)(at + T::at(8, nch, T::VGAP)));
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(uintptr_t)(at + T::at(8, vp, T::VGAP)));
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
@@ -351,13 +392,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
         }
     };
     auto largest = [&](const f32x16(&sc)[KB]) __attribute__((always_inline)) {
-        float x = fmaxf(sc[0][0], sc[0][1]);
+        float x = sc[0][0];  // (a NaN among them stays: the row is NaN)
 #pragma unroll
-        for (int e = 2; e < 16; ++e) x = fmaxf(x, sc[0][e]);
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int kb = 1; kb < KB; ++kb)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x = fmaxf(x, sc[kb][e]);
+            for (int e = 0; e < 16; ++e) x = __builtin_elementwise_maximum(x, sc[kb][e]);
         return xmax32(x);
     };
     // the running maximum takes in a tile's; O and the sum follow only where some row's grew by more than 2^8
@@ -365,7 +404,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
         if (__builtin_amdgcn_ballot_w64((mloc - m) * c > 8.0f)) {
             const float mnew = fmaxf(m, mloc);
             const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mnew) * c);
-            lsum *= alpha;
+            if (!T::ONES) lsum *= alpha;
 #pragma unroll
             for (int i = 0; i < NDB; ++i) o[i] *= alpha;
             m = mnew;
@@ -391,7 +430,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
                 pk[2 * kb + (e >> 3)][e & 7] = f2bf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][e], cf, -mc)));
         // the rounded weights are summed: where one weight is nearly all, its rounding divides out
 #pragma unroll
-        for (int i = 0; i < 2 * KB; ++i) {
+        for (int i = 0; i < (T::ONES ? 0 : 2 * KB); ++i) {
             const bf16x2 one = {1.0f, 1.0f};
             lsum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 0, 1), one, lsum, false);
             lsum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(pk[i], pk[i], 2, 3), one, lsum, false);
@@ -406,52 +445,91 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
             for (int db = 0; db < NDB; ++db)
                 o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfrag(so, i, db), pk[i], o[db], 0, 0, 0);
     };
-    // this wave's part of the next tile has landed and its LDS reads are done; then everybody's
-    auto meet = [&]() __attribute__((always_inline)) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // This wave's part of what the tile needs has landed, and its LDS reads are done; then everybody's. The copies of
+    // `later` more tiles may still be on their way (a wave's copies land in order).
+    constexpr int MINE = GEN ? 0 : T::NPK / NW + T::NPV / NW;
+    auto meet = [&](bool later) __attribute__((always_inline)) {
+        if (NS > 2 && later)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * MINE) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    // Tile t's weights and products beside tile t + 1's scores, which do not depend on them: the matrix pipe has work
-    // while a wave's vector instructions run. K runs one tile ahead of V, each in two slots of its own.
-    auto step = [&](auto cut_c, int t, f32x16(&s0)[KB], f32x16(&s1)[KB], const unsigned even, const unsigned odd)
-        __attribute__((always_inline)) {
-        constexpr bool CUT = decltype(cut_c)::value;
-        meet();
-        if (t + 2 < nkt) issue(std::false_type{}, t + 2, even);
-        if (t + 1 < nkt) issue(std::true_type{}, t + 1, odd);
-        bf16x8 pk[2 * KB];
-        if (!CUT || t + 1 < nkt) qk(s1, odd);
-        weigh(s0, pk);
-        pv(pk, even);
-        if (!CUT || t + 1 < nkt) {
-            score(cut_c, s1, t + 1);
-            const float mloc = largest(s1);
-            raise(mloc, s1);
-        }
+    constexpr std::false_type K{};
+    constexpr std::true_type V{};
+    auto next = [](unsigned slot) __attribute__((always_inline)) {
+        return slot == (unsigned)(NS - 1) * T::BYTES ? 0u : slot + T::BYTES;
     };
     if (NW > 4 && wave >= NW / 2) __builtin_amdgcn_s_setprio(1);
-    if (nkt > 0) {
-        meet();
-        if (nkt > 1) issue(std::false_type{}, 1, T::BYTES);
-        issue(std::true_type{}, 0, 0);
-        qk(sa, 0);
-        score(std::true_type{}, sa, 0);
-        raise(largest(sa), sa);
-    }
     int t = 0;
-    for (; t + 2 < nfull; t += 2) {  // two a turn: the slots are constants
-        step(std::false_type{}, t, sa, sb, 0, T::BYTES);
-        step(std::false_type{}, t + 1, sb, sa, T::BYTES, 0);
-    }
-    for (; t < nkt; ++t) {
-        const unsigned even = t & 1 ? T::BYTES : 0;
-        step(std::true_type{}, t, sa, sb, even, T::BYTES - even);
+    unsigned now = 0, free = (NS - 1) * T::BYTES;  // tile t's slot, and that of tile t - 1
+    if constexpr (!AHEAD) {
+        auto step = [&](auto cut_c) __attribute__((always_inline)) {
+            meet(t + NS - 2 < nkt);
+            if (t + NS - 1 < nkt) issue(K, t + NS - 1, free), issue(V, t + NS - 1, free);
+            bf16x8 pk[2 * KB];
+            qk(sa, now);
+            score(cut_c, sa, t);
+            raise(largest(sa), sa);
+            weigh(sa, pk);
+            pv(pk, now);
+            free = now, now = next(now), ++t;
+        };
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) sa[kb] = sb[kb];
+        for (int i = 0; i < NS - 1; ++i)
+            if (i < nkt) {
+                if (i > 0) issue(K, i, i * T::BYTES);
+                issue(V, i, i * T::BYTES);
+            }
+#pragma unroll 1
+        while (t < nfull) step(std::false_type{});
+#pragma unroll 1
+        while (t < nkt) step(std::true_type{});
+    } else {
+        // Tile t's weights and products beside tile t + 1's scores, which do not depend on them: the matrix pipe has
+        // work while a wave's vector instructions run. K runs one tile ahead of V.
+        auto step = [&](auto cut_c, f32x16(&s0)[KB], f32x16(&s1)[KB]) __attribute__((always_inline)) {
+            constexpr bool CUT = decltype(cut_c)::value;
+            const unsigned then = next(now);
+            meet(t + NS - 1 < nkt);
+            if (t + NS < nkt) issue(K, t + NS, now);
+            if (t + NS - 1 < nkt) issue(V, t + NS - 1, free);
+            bf16x8 pk[2 * KB];
+            if (!CUT || t + 1 < nkt) qk(s1, then);
+            weigh(s0, pk);
+            pv(pk, now);
+            if (!CUT || t + 1 < nkt) {
+                score(cut_c, s1, t + 1);
+                raise(largest(s1), s1);
+            }
+            free = now, now = then, ++t;
+        };
+        if (nkt > 0) {
+            meet(false);
+#pragma unroll
+            for (int i = 1; i < NS; ++i) {
+                if (i < nkt) issue(K, i, i * T::BYTES);
+                if (i - 1 < nkt) issue(V, i - 1, (i - 1) * T::BYTES);
+            }
+            qk(sa, 0);
+            score(std::true_type{}, sa, 0);
+            raise(largest(sa), sa);
+        }
+#pragma unroll 1
+        while (t + 2 < nfull) {
+            step(std::false_type{}, sa, sb);
+            step(std::false_type{}, sb, sa);
+        }
+#pragma unroll 1
+        while (t < nkt) {
+            step(std::true_type{}, sa, sb);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) sa[kb] = sb[kb];
+        }
     }
 
-    const float l = xsum32(lsum);
+    const float l = T::ONES ? o[HD / 32][4 * (HD % 32 / 8)] : xsum32(lsum);
     const float inv = hi > 0 ? 1.0f / l : 0.f;  // a row that sees nothing is 0
     if constexpr (SPLIT) {
         if (fr < flat) {
@@ -597,13 +675,15 @@ struct Plan {
     size_t stat, ws;
 };
 
-constexpr int NWL = 8, MINW1 = 3, WANT = 2048;
+constexpr int NW64 = 4, MW64 = 3, NS64 = 2, NW72 = 4, MW72 = 3, NS72 = 2, NW128 = 4, MW128 = 2, NS128 = 2, NW256 = 4, MW256 = 2, NS256 = 2;
+constexpr bool AH64 = false, AH72 = false, AH128 = true, AH256 = false;
+constexpr int MINW1 = 3, WANT = 2048, SORTED = 512;
 
 Plan make_plan(int n, int rows_q, int rows_k, int Hkv, int group, int hd, int max_rows) {
     Plan p{};
     const long mean = n ? (long)rows_q * group / n : 0;
-    p.NW = mean <= 48 ? 1 : NWL;
-    p.per_log2 = p.NW == 1 ? 5 : 8;
+    p.NW = mean <= 48 ? 1 : hd <= 64 ? NW64 : hd <= 80 ? NW72 : hd <= 128 ? NW128 : NW256;
+    p.per_log2 = p.NW == 1 ? 5 : p.NW == 4 ? 7 : 8;
     long nslots = ((long)rows_q * group >> p.per_log2) + n;
     const long mr = (long)max_rows * group;
     const long blocks = nslots * Hkv;
@@ -622,25 +702,25 @@ Plan make_plan(int n, int rows_q, int rows_k, int Hkv, int group, int hd, int ma
     return p;
 }
 
-template <int HD, bool GEN, int NW, int MINW, bool SPLIT>
+template <int HD, bool GEN, int NW, int MINW, int NS, bool AHEAD, bool SPLIT>
 void launch_docs(const DocsArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)(a.nslots * a.Hkv)), block(NW * 64);
     switch ((a.cap_log2 != 0.f ? 1 : 0) | (a.slopes ? 2 : 0)) {
-        case 0: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, SPLIT, 0>), grid, block, 0, s, a); break;
-        case 1: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, SPLIT, 1>), grid, block, 0, s, a); break;
-        case 2: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, SPLIT, 2>), grid, block, 0, s, a); break;
-        default: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, SPLIT, 3>), grid, block, 0, s, a);
+        case 0: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, NS, AHEAD, SPLIT, 0>), grid, block, 0, s, a); break;
+        case 1: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, NS, AHEAD, SPLIT, 1>), grid, block, 0, s, a); break;
+        case 2: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, NS, AHEAD, SPLIT, 2>), grid, block, 0, s, a); break;
+        default: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, NS, AHEAD, SPLIT, 3>), grid, block, 0, s, a);
     }
 }
 
-template <int HD, bool GEN, int MINW>
+template <int HD, bool GEN, int NW, int MINW, int NS, bool AHEAD>
 void launch_width(const DocsArgs& a, const Plan& p, hipStream_t s) {
     if (p.split)
-        launch_docs<HD, GEN, 1, MINW1, true>(a, s);
+        launch_docs<HD, GEN, 1, MINW1, 2, false, true>(a, s);
     else if (p.NW == 1)
-        launch_docs<HD, GEN, 1, MINW1, false>(a, s);
+        launch_docs<HD, GEN, 1, MINW1, 2, false, false>(a, s);
     else
-        launch_docs<HD, GEN, NWL, MINW, false>(a, s);
+        launch_docs<HD, GEN, NW, MINW, NS, AHEAD, false>(a, s);
 }
 
 int check_docs(int n, int rows_q, int rows_k, int Hq, int Hkv, int hd, int max_rows) {
@@ -688,24 +768,24 @@ extern "C" int mme_attention_docs(const void* q, long ldq, const void* k, long l
     a.qoff = q_offsets, a.koff = k_offsets, a.prefix = prefix, a.slopes = slopes, a.part = (float*)workspace, a.stat = a.part + p.stat;
     a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldo = ldo, a.nslots = p.nslots;
     a.n = n, a.rows_q = rows_q, a.rows_k = rows_k, a.Hkv = Hkv, a.group = Hq / Hkv, a.hd = hd;
-    a.max_rows = mr, a.causal = causal ? 1 : 0, a.per_log2 = p.per_log2, a.part_rows = p.part_rows;
+    a.sorted = !p.split && n > 1 && n <= 63 && (long)p.nslots * Hkv >= SORTED, a.max_rows = mr, a.causal = causal ? 1 : 0, a.per_log2 = p.per_log2, a.part_rows = p.part_rows;
     a.scale_log2 = scale * LOG2E;
     a.cap_log2 = softcap * LOG2E;
     a.cap_in = softcap != 0.f ? 2.0f * a.scale_log2 / softcap : 0.f;
     hipStream_t s = as_stream(stream);
     switch (hd) {
-        case 64: launch_width<64, false, 3>(a, p, s); break;
-        case 72: launch_width<72, false, 3>(a, p, s); break;
-        case 80: launch_width<80, false, 3>(a, p, s); break;
-        case 128: launch_width<128, false, 2>(a, p, s); break;
-        case 256: launch_width<256, false, 2>(a, p, s); break;
+        case 64: launch_width<64, false, NW64, MW64, NS64, AH64>(a, p, s); break;
+        case 72: launch_width<72, false, NW72, MW72, NS72, AH72>(a, p, s); break;
+        case 80: launch_width<80, false, NW72, MW72, NS72, AH72>(a, p, s); break;
+        case 128: launch_width<128, false, NW128, MW128, NS128, AH128>(a, p, s); break;
+        case 256: launch_width<256, false, NW256, MW256, NS256, AH256>(a, p, s); break;
         default:
             if (hd < 64)
-                launch_width<64, true, 2>(a, p, s);
+                launch_width<64, true, NW64, 2, 2, false>(a, p, s);
             else if (hd < 128)
-                launch_width<128, true, 2>(a, p, s);
+                launch_width<128, true, NW128, 2, 2, false>(a, p, s);
             else
-                launch_width<256, true, 1>(a, p, s);
+                launch_width<256, true, NW256, NW256 / 4, 2, false>(a, p, s);
     }
     if (p.split) {
         if (int rc = mme_check_launch("mme_attention_docs")) return rc;
