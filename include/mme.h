@@ -405,13 +405,13 @@ int mme_rope_axes(const void* x, long ldx, void* y, long ldy, int rows, int nhea
  * [k_offsets[d], k_offsets[d+1]); the offsets (int32[n+1], not decreasing; clamped to the rows there are) may be the
  * same array. Query i of a document stands at key position p = i + klen - qlen. It sees key j of its own document
  * where  !causal,  or j <= p,  or j < prefix[d] (int32[n], nullable, with causal only). Its score is
- *   x = scale q.k;  softcap > 0: x = softcap tanh(x / softcap);  slopes (fp32[Hq], nullable): x -= slopes[h] |p - j|
+ *   x = scale q.k;  softcap (0, or 1e-3 .. 1e3): x = softcap tanh(x / softcap);  slopes (fp32[Hq], nullable): x -= slopes[h] |p - j|
  * and out = softmax(x) v over the keys it sees, 0 where it sees none. A key that a query does not see adds nothing
  * to it, whatever k and v hold there. Rows of no document are left as they were, and so are a document's rows from
  * max_rows on (max_rows: the most query rows a document has, or rows_q; small ones let long keys be split over the
  * device and joined). q: bf16 [rows_q, ldq], head h at column h*hd; k, v: bf16 [rows_k, ld], key head h / (Hq/Hkv);
  * out: bf16 [rows_q, ldo]. hd: multiples of 8 up to 128, of 16 up to 256. 16-byte aligned pointers, leading dims
- * % 8 == 0. fp32 scores, softmax and sums; the weights are rounded to bf16 for the matrix instruction.
+ * % 8 == 0, those of k and v under 2^24. fp32 scores, softmax and sums; the weights are rounded to bf16 for the matrix instruction.
  * workspace >= mme_attention_docs_workspace_bytes(...) (0: may be null). */
 size_t mme_attention_docs_workspace_bytes(int n, int rows_q, int rows_k, int Hq, int Hkv, int hd, int max_rows);
 int mme_attention_docs(const void* q, long ldq, const void* k, long ldk, const void* v, long ldv, void* out, long ldo,

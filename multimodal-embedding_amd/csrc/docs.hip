@@ -41,9 +41,8 @@ struct DocsArgs {
     const float* slopes;
     float *part, *stat;  // split: O [slot][key head][flat row][hd], and (maximum, sum) [slot][key head][flat row][2]
     long ldq, ldk, ldv, ldo;
-    int nslots, n, rows_q, rows_k, Hkv, group, hd, max_rows, causal, part_rows;
-    int sorted;
-    int per_log2;       // a slot's flat rows, or keys (split), are 1 << per_log2
+    int nslots, n, rows_q, rows_k, Hkv, group, hd, max_rows, causal, part_rows, row_blocks, sorted;
+    int per;            // a slot's flat rows (a power of two), or keys (split)
     float scale_log2, cap_log2, cap_in;
 };
 
@@ -55,17 +54,20 @@ __device__ __forceinline__ float xsum32(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// 16 bytes a lane from base + off to LDS at `at` (wave-uniform, as base is) + 16 lane, retired by the caller's wait
+// 16 bytes a lane from base + off to LDS at `at` (wave-uniform, as base is) + 16 lane, retired by the caller's wait.
+// The wait states cover an M0 write, and base in SGPRs that a vector instruction (a spill's reload) has just written.
 __device__ __forceinline__ void dma16(const char* base, unsigned off, unsigned at) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(at) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(at) : "memory", "m0");
 }
 __device__ __forceinline__ int clamp_row(int x, int rows) { return min(max(x, 0), rows); }
 
-// Work is dealt out in slots of `1 << sh` units (flat rows, or keys). Document d owns the slots from
-// (off[d] * mul >> sh) + d on: that many always hold its units, because rounding down loses less than the one slot
-// that `+ d` adds, so a slot finds its document by a search in `off` and no table is needed. Surplus slots end at
-// once. Offsets are clamped to [0, rows]: wrong ones give wrong rows, never a wrong address.
-__device__ __forceinline__ int first_slot(int off, int d, int mul, int sh) { return (int)(((long)off * mul >> sh) + d); }
+// Work is dealt out in slots of `per` units (flat rows, or keys). Document d owns the slots from off[d] * mul / per + d
+// on: that many always hold its units, because rounding down loses less than the one slot that `+ d` adds, so a slot
+// finds its document by a search in `off` and no table is needed. Surplus slots end at once. Offsets are clamped to
+// [0, rows]: wrong ones give wrong rows, never a wrong address.
+__device__ __forceinline__ int first_slot(int off, int d, int mul, int per) {
+    return (int)((unsigned)off * (unsigned)mul / (unsigned)per) + d;  // off * mul < 2^31
+}
 
 struct Doc {
     int d, q0, qlen, k0, klen, pre, first;
@@ -81,7 +83,7 @@ __device__ __forceinline__ Doc find_doc(const DocsArgs& a, int slot) {
     while (hi - lo > 63) {  // 64 documents a step
         const int step = (hi - lo + 63) >> 6;
         const int i = lo + lane * step;
-        const bool le = i < hi && first_slot(clamp_row(off[min(i, a.n)], rows), i, mul, a.per_log2) <= slot;
+        const bool le = i < hi && first_slot(clamp_row(off[min(i, a.n)], rows), i, mul, a.per) <= slot;
         const int c = __popcll(__builtin_amdgcn_ballot_w64(le));
         if (c > 0) lo += (c - 1) * step;
         hi = min(hi, lo + step);
@@ -92,10 +94,10 @@ __device__ __forceinline__ Doc find_doc(const DocsArgs& a, int slot) {
     const int i = min(lo + lane, a.n);
     const int qo = clamp_row(a.qoff[i], a.rows_q), ko = clamp_row(a.koff[i], a.rows_k);
     const int pr = a.prefix ? a.prefix[min(i, a.n - 1)] : 0;
-    int fs = first_slot(SPLIT ? ko : qo, i, mul, a.per_log2), l;
+    int fs = first_slot(SPLIT ? ko : qo, i, mul, a.per), l;
     if (SORT && a.sorted) {
         const int kl = lane < a.n ? __shfl_down(ko, 1, 64) - ko : -1;
-        const int parts = lane < a.n ? (min(max(__shfl_down(qo, 1, 64) - qo, 0), a.max_rows) * mul + (1 << a.per_log2) - 1) >> a.per_log2 : 0;
+        const int parts = lane < a.n ? (min(max(__shfl_down(qo, 1, 64) - qo, 0), a.max_rows) * mul + a.per - 1) / a.per : 0;
         fs = 0;  // the slots of the documents before this lane's
         for (int j = 0; j < a.n; ++j) {
             const int kj = __builtin_amdgcn_readlane(kl, j), pj = __builtin_amdgcn_readlane(parts, j);
@@ -194,14 +196,14 @@ __device__ __forceinline__ void row_alone(const DocsArgs& a, const Doc& D, int g
 }
 
 // MODE: 1 = capped scores, 2 = biased by distance, 3 = both
-// AHEAD: the next tile's scores are formed beside this one's weights; NS: slots of the ring
-template <int HD, bool GEN, int NW, int MINW, int NS, bool AHEAD, bool SPLIT, int MODE>
+// AHEAD: the next tile's scores are formed beside this one's weights
+template <int HD, bool GEN, int NW, int MINW, bool AHEAD, bool SPLIT, int MODE>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW))) void attn_docs_kernel(DocsArgs a) {
     using T = Tile<HD, GEN>;
     constexpr int KT = T::KT, KB = T::KB, NKS = T::NKS, NDB = T::NDB, QB = NW * 32;
     constexpr bool HALF = GEN || HD % 16 != 0;  // the last k-step may reach past the head dim
-    constexpr int ZERO = NS * T::BYTES;           // 16 zero bytes for it
-    __shared__ __attribute__((aligned(16))) char lds[NS * T::BYTES + (HALF ? 16 : 0)];
+    constexpr int ZERO = 2 * T::BYTES;           // 16 zero bytes for it
+    __shared__ __attribute__((aligned(16))) char lds[2 * T::BYTES + (HALF ? 16 : 0)];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -210,13 +212,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     // rows lie in shared lines; else an XCD keeps to as few key heads as it can, whose K / V its slots share, and takes
     // their slots side by side, so that all heads' first slots (the longest, where they are sorted) start first.
     constexpr bool OWN = SPLIT || NW == 1;
-    int slot, kvh;
+    int slot, kvh, rb = 0;
     {
         const int bid = blockIdx.x, nwg = gridDim.x;
         const int xcd = bid & 7, loc = bid >> 3, q8 = nwg >> 3, r8 = nwg & 7;
         const int id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + loc;
-        if (OWN)
-            slot = id / a.Hkv, kvh = id - slot * a.Hkv;
+        if (OWN) {
+            const int x = SPLIT ? id / a.row_blocks : id;  // split: the blocks of rows of one chunk side by side too
+            rb = id - x * (SPLIT ? a.row_blocks : 1), slot = x / a.Hkv, kvh = x - slot * a.Hkv;
+        }
         else if ((a.Hkv & 7) == 0)
             slot = loc / (a.Hkv >> 3), kvh = xcd * (a.Hkv >> 3) + loc - slot * (a.Hkv >> 3);
         else
@@ -226,24 +230,24 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     const int qlen = D.qlen, klen = D.klen;
     const int flat = min(qlen, a.max_rows) * a.group;  // flat rows of this document
     int part = slot - D.first;
-    const int chunk = 1 << a.per_log2;
-    const int nparts = (int)(((SPLIT ? (long)klen : (long)flat) + chunk - 1) >> a.per_log2);
+    const int nparts = (int)(((unsigned)(SPLIT ? klen : flat) + (unsigned)a.per - 1) / (unsigned)a.per);
     if (part < 0 || part >= nparts || flat == 0) return;
     if (!SPLIT && a.causal) part = nparts - 1 - part;  // the rows with the most keys first
 
-    const int f0 = SPLIT ? 0 : part * QB;                       // the block's first flat row
+    const int f0 = SPLIT ? rb * QB : part * QB;                 // the block's first flat row
+    if (SPLIT && f0 >= flat) return;
     const int fr = f0 + wave * 32 + r;                          // this lane's
     const int qi = min(fr, flat - 1) / a.group, gh = kvh * a.group + min(fr, flat - 1) - qi * a.group;
     const int pq = qi + klen - qlen;                            // its place among the keys
     const int hi = a.causal ? min(klen, max(D.pre, pq + 1)) : klen;  // it sees keys [0, hi)
-    const int key_lo = SPLIT ? part << a.per_log2 : 0;
+    const int key_lo = SPLIT ? part * a.per : 0;
     // the block's first row sees the fewest keys, its last row the most
     const int q_first = f0 / a.group, q_last = (min(f0 + QB, flat) - 1) / a.group;
     int hi_min = a.causal ? min(klen, max(D.pre, q_first + klen - qlen + 1)) : klen;
     int hi_max = a.causal ? min(klen, max(D.pre, q_last + klen - qlen + 1)) : klen;
     if (SPLIT) {
-        hi_min = min((long)hi_min, (long)key_lo + chunk);
-        hi_max = min((long)hi_max, (long)key_lo + chunk);
+        hi_min = min((long)hi_min, (long)key_lo + a.per);
+        hi_max = min((long)hi_max, (long)key_lo + a.per);
     }
     const int nfull = (hi_min - key_lo) / KT;  // tiles that every row sees whole (none where negative)
     const int nkt = hi_max > key_lo ? (hi_max - key_lo + KT - 1) / KT : 0;
@@ -259,7 +263,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     // A lane's places in them are the same in every tile but one that reaches past the document.
     const int npk = GEN ? nch * KT / 64 : T::NPK, npv = GEN ? nch * KT / 64 : T::NPV;
     if (T::ONES)
-        for (int i = tid; i < NS * KT; i += NW * 64)
+        for (int i = tid; i < 2 * KT; i += NW * 64)
             *reinterpret_cast<u16x8*>(lds + i / KT * T::BYTES + T::VOFF + (i % KT * T::VP + HD / 8) * 16) =
                 u16x8{0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80};
     auto row_of = [&](bool isV, int i) __attribute__((always_inline)) { return ((wave + NW * i) * 64 + lane) / (isV ? vp : kp); };
@@ -445,87 +449,73 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
             for (int db = 0; db < NDB; ++db)
                 o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfrag(so, i, db), pk[i], o[db], 0, 0, 0);
     };
-    // This wave's part of what the tile needs has landed, and its LDS reads are done; then everybody's. The copies of
-    // `later` more tiles may still be on their way (a wave's copies land in order).
-    constexpr int MINE = GEN ? 0 : T::NPK / NW + T::NPV / NW;
-    auto meet = [&](bool later) __attribute__((always_inline)) {
-        if (NS > 2 && later)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * MINE) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // this wave's part of the next tile has landed and its LDS reads are done; then everybody's
+    auto meet = [&]() __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    constexpr std::false_type K{};
-    constexpr std::true_type V{};
-    auto next = [](unsigned slot) __attribute__((always_inline)) {
-        return slot == (unsigned)(NS - 1) * T::BYTES ? 0u : slot + T::BYTES;
-    };
-    if (NW > 4 && wave >= NW / 2) __builtin_amdgcn_s_setprio(1);
+    constexpr std::false_type K{}, WHOLE{};
+    constexpr std::true_type V{}, CUT{};
     int t = 0;
-    unsigned now = 0, free = (NS - 1) * T::BYTES;  // tile t's slot, and that of tile t - 1
-    if constexpr (!AHEAD) {
-        auto step = [&](auto cut_c) __attribute__((always_inline)) {
-            meet(t + NS - 2 < nkt);
-            if (t + NS - 1 < nkt) issue(K, t + NS - 1, free), issue(V, t + NS - 1, free);
-            bf16x8 pk[2 * KB];
-            qk(sa, now);
-            score(cut_c, sa, t);
-            raise(largest(sa), sa);
-            weigh(sa, pk);
-            pv(pk, now);
-            free = now, now = next(now), ++t;
+    unsigned now = 0, other = T::BYTES;  // tile t's slot, and the other
+    if (nkt > 0) {
+        if (!AHEAD) issue(V, 0, 0);
+        auto turn = [&]() __attribute__((always_inline)) {
+            const unsigned x = now;
+            now = other, other = x, ++t;
         };
-#pragma unroll
-        for (int i = 0; i < NS - 1; ++i)
-            if (i < nkt) {
-                if (i > 0) issue(K, i, i * T::BYTES);
-                issue(V, i, i * T::BYTES);
-            }
+        if constexpr (!AHEAD) {
+            auto step = [&](auto cut_c) __attribute__((always_inline)) {
+                meet();
+                if (t + 1 < nkt) issue(K, t + 1, other), issue(V, t + 1, other);
+                bf16x8 pk[2 * KB];
+                qk(sa, now);
+                score(cut_c, sa, t);
+                raise(largest(sa), sa);
+                weigh(sa, pk);
+                pv(pk, now);
+                turn();
+            };
 #pragma unroll 1
-        while (t < nfull) step(std::false_type{});
+            while (t < nfull) step(WHOLE);
 #pragma unroll 1
-        while (t < nkt) step(std::true_type{});
-    } else {
-        // Tile t's weights and products beside tile t + 1's scores, which do not depend on them: the matrix pipe has
-        // work while a wave's vector instructions run. K runs one tile ahead of V.
-        auto step = [&](auto cut_c, f32x16(&s0)[KB], f32x16(&s1)[KB]) __attribute__((always_inline)) {
-            constexpr bool CUT = decltype(cut_c)::value;
-            const unsigned then = next(now);
-            meet(t + NS - 1 < nkt);
-            if (t + NS < nkt) issue(K, t + NS, now);
-            if (t + NS - 1 < nkt) issue(V, t + NS - 1, free);
-            bf16x8 pk[2 * KB];
-            if (!CUT || t + 1 < nkt) qk(s1, then);
-            weigh(s0, pk);
-            pv(pk, now);
-            if (!CUT || t + 1 < nkt) {
-                score(cut_c, s1, t + 1);
-                raise(largest(s1), s1);
-            }
-            free = now, now = then, ++t;
-        };
-        if (nkt > 0) {
-            meet(false);
-#pragma unroll
-            for (int i = 1; i < NS; ++i) {
-                if (i < nkt) issue(K, i, i * T::BYTES);
-                if (i - 1 < nkt) issue(V, i - 1, (i - 1) * T::BYTES);
-            }
+            while (t < nkt) step(CUT);
+        } else {
+            // Tile t's weights and products beside tile t + 1's scores, which do not depend on them: the matrix pipe
+            // has work while the wave's vector instructions run. K runs one tile ahead of V.
+            auto step = [&](auto cut_c, f32x16(&s0)[KB], f32x16(&s1)[KB]) __attribute__((always_inline)) {
+                const bool more = !decltype(cut_c)::value || t + 1 < nkt;
+                meet();
+                if (t + 2 < nkt) issue(K, t + 2, now);
+                if (t + 1 < nkt) issue(V, t + 1, other);
+                bf16x8 pk[2 * KB];
+                if (more) qk(s1, other);
+                weigh(s0, pk);
+                pv(pk, now);
+                if (more) {
+                    score(cut_c, s1, t + 1);
+                    raise(largest(s1), s1);
+                }
+                turn();
+            };
+            meet();
+            if (nkt > 1) issue(K, 1, other);
+            issue(V, 0, 0);
             qk(sa, 0);
-            score(std::true_type{}, sa, 0);
+            score(CUT, sa, 0);
             raise(largest(sa), sa);
-        }
 #pragma unroll 1
-        while (t + 2 < nfull) {
-            step(std::false_type{}, sa, sb);
-            step(std::false_type{}, sb, sa);
-        }
+            while (t + 2 < nfull) {
+                step(WHOLE, sa, sb);
+                step(WHOLE, sb, sa);
+            }
 #pragma unroll 1
-        while (t < nkt) {
-            step(std::true_type{}, sa, sb);
+            while (t < nkt) {
+                step(CUT, sa, sb);
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) sa[kb] = sb[kb];
+                for (int kb = 0; kb < KB; ++kb) sa[kb] = sb[kb];
+            }
         }
     }
 
@@ -594,7 +584,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
         const int fx = f0 + wave * 32 + x, qx = fx / a.group, gx = kvh * a.group + fx - qx * a.group, px = qx + klen - qlen;
         const int hx = min(klen, max(D.pre, px + 1));
         float mx, lx, acc[(HD + 63) / 64];
-        row_alone<HD>(a, D, gx, kvh, px, qx, key_lo, SPLIT ? (int)min((long)hx, (long)key_lo + chunk) : hx, mx, lx, acc);
+        row_alone<HD>(a, D, gx, kvh, px, qx, key_lo, SPLIT ? (int)min((long)hx, (long)key_lo + a.per) : hx, mx, lx, acc);
         const long at = ((long)slot * a.Hkv + kvh) * a.part_rows + fx;
         if (SPLIT && lane == 0) a.stat[2 * at] = mx, a.stat[2 * at + 1] = lx;
 #pragma unroll
@@ -622,8 +612,8 @@ __global__ __launch_bounds__(256) void join_docs_kernel(DocsArgs a) {
     const int qi = fr / a.group, gh = kvh * a.group + fr % a.group;
     const int pre = a.prefix ? min(max(a.prefix[d], 0), klen) : 0;
     const int hi = a.causal ? min(klen, max(pre, qi + klen - qlen + 1)) : klen;
-    const int nparts = (int)(((long)klen + (1 << a.per_log2) - 1) >> a.per_log2);
-    const long row = ((long)first_slot(k0, d, 1, a.per_log2) * a.Hkv + kvh) * a.part_rows + fr;
+    const int nparts = (int)(((unsigned)klen + (unsigned)a.per - 1) / (unsigned)a.per);
+    const long row = ((long)first_slot(k0, d, 1, a.per) * a.Hkv + kvh) * a.part_rows + fr;
     const long step = (long)a.Hkv * a.part_rows;
     const float2* stat = reinterpret_cast<const float2*>(a.stat) + row;
     float m = -INFINITY;
@@ -671,56 +661,64 @@ __global__ __launch_bounds__(256) void join_docs_kernel(DocsArgs a) {
 
 struct Plan {
     bool split;
-    int NW, per_log2, part_rows, nslots;
+    int NW, per, part_rows, row_blocks, nslots;
     size_t stat, ws;
 };
 
-constexpr int NW64 = 4, MW64 = 3, NS64 = 2, NW72 = 4, MW72 = 3, NS72 = 2, NW128 = 4, MW128 = 2, NS128 = 2, NW256 = 4, MW256 = 2, NS256 = 2;
-constexpr bool AH64 = false, AH72 = false, AH128 = true, AH256 = false;
-constexpr int MINW1 = 3, WANT = 2048, SORTED = 512;
-
+// How the work is cut, from the sizes alone (the lengths are on the device).
 Plan make_plan(int n, int rows_q, int rows_k, int Hkv, int group, int hd, int max_rows) {
     Plan p{};
-    const long mean = n ? (long)rows_q * group / n : 0;
-    p.NW = mean <= 48 ? 1 : hd <= 64 ? NW64 : hd <= 80 ? NW72 : hd <= 128 ? NW128 : NW256;
-    p.per_log2 = p.NW == 1 ? 5 : p.NW == 4 ? 7 : 8;
-    long nslots = ((long)rows_q * group >> p.per_log2) + n;
-    const long mr = (long)max_rows * group;
-    const long blocks = nslots * Hkv;
-    if (n && mr <= 32 && rows_k / n > 256 && blocks < 2048) {
+    if (n == 0 || max_rows == 0) return p;
+    const long flat = (long)rows_q * group, keys = (long)rows_k / n;
+    // One wave a workgroup where documents fill no more than one and there are workgroups enough; else four, also
+    // where three of them only help to copy. 12 000 rows in documents of 16 / 32 / 48 rows, 12 heads of 64: one wave
+    // 42 / 26 / 29 us, four 51 / 29 / 23; one key head of 256 (32 flat rows) 79 and 46.
+    p.NW = flat / n <= 32 && hd <= 128 && (flat / 32 + n) * Hkv >= 512 ? 1 : 4;
+    p.per = p.NW * 32;
+    p.row_blocks = 1;
+    long nslots = flat / p.per + n;
+    // Few flat rows a document: its keys in parts, for nearly three rounds of the workgroups that fit the device by
+    // their LDS (documents of different lengths at just over two rounds 195 us, at 2.7 157: the last is half empty).
+    // Two parts at least, and enough for a workgroup to read without: one query against 512 / 1 024 / 4 096 keys of 8
+    // documents, 8 heads of 128, whole 14.9 / 23 / 81 us, in parts 14.7 / 17 / 43; 16 documents, 16 heads of 72, 1 024 /
+    // 4 096 keys 21 / 85 and 25 / 71 (more workgroups need longer documents). Documents of 1 353 keys on average, 256
+    // to 4 096, 64 x 16 heads of 72: 119 and 100 us.
+    const long mr = (long)max_rows * group, rb = (mr + 31) / 32, blocks = nslots * Hkv;
+    const long resident = 256 * (hd <= 64 ? 4 : hd <= 80 ? 3 : 2);
+    const long parts = resident * 11 / 4 / (n * Hkv * rb);
+    if (mr <= 256 && parts >= 2 && keys * hd >= (blocks <= 128 ? 40960 : 81920)) {
         p.split = true;
         p.NW = 1;
-        const long want = (WANT + Hkv - 1) / Hkv;  // chunks in all
-        p.per_log2 = hd > 128 ? 5 : 6;  // at least a tile
-        while (((long)rows_k >> p.per_log2) > want) ++p.per_log2;
-        p.part_rows = (int)mr;
-        nslots = ((long)rows_k >> p.per_log2) + n;
+        const long kt = hd > 128 ? 32 : 64;  // keys a tile
+        p.per = (int)((keys + parts * kt - 1) / (parts * kt) * kt);
+        p.part_rows = (int)mr, p.row_blocks = (int)rb;
+        nslots = (long)rows_k / p.per + n;
         p.stat = (size_t)nslots * Hkv * mr * hd;  // where the statistics begin, in floats
         p.ws = (p.stat + (size_t)nslots * Hkv * mr * 2) * 4;
     }
-    p.nslots = nslots * Hkv < (1L << 31) ? (int)nslots : -1;
+    p.nslots = nslots * Hkv * p.row_blocks < (1L << 31) ? (int)nslots : -1;
     return p;
 }
 
-template <int HD, bool GEN, int NW, int MINW, int NS, bool AHEAD, bool SPLIT>
+template <int HD, bool GEN, int NW, int MINW, bool AHEAD, bool SPLIT>
 void launch_docs(const DocsArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)(a.nslots * a.Hkv)), block(NW * 64);
+    const dim3 grid((unsigned)(a.nslots * a.Hkv * a.row_blocks)), block(NW * 64);
     switch ((a.cap_log2 != 0.f ? 1 : 0) | (a.slopes ? 2 : 0)) {
-        case 0: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, NS, AHEAD, SPLIT, 0>), grid, block, 0, s, a); break;
-        case 1: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, NS, AHEAD, SPLIT, 1>), grid, block, 0, s, a); break;
-        case 2: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, NS, AHEAD, SPLIT, 2>), grid, block, 0, s, a); break;
-        default: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, NS, AHEAD, SPLIT, 3>), grid, block, 0, s, a);
+        case 0: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, AHEAD, SPLIT, 0>), grid, block, 0, s, a); break;
+        case 1: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, AHEAD, SPLIT, 1>), grid, block, 0, s, a); break;
+        case 2: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, AHEAD, SPLIT, 2>), grid, block, 0, s, a); break;
+        default: hipLaunchKernelGGL((attn_docs_kernel<HD, GEN, NW, MINW, AHEAD, SPLIT, 3>), grid, block, 0, s, a);
     }
 }
 
-template <int HD, bool GEN, int NW, int MINW, int NS, bool AHEAD>
+template <int HD, bool GEN, int MINW, bool AHEAD>
 void launch_width(const DocsArgs& a, const Plan& p, hipStream_t s) {
     if (p.split)
-        launch_docs<HD, GEN, 1, MINW1, 2, false, true>(a, s);
-    else if (p.NW == 1)
-        launch_docs<HD, GEN, 1, MINW1, 2, false, false>(a, s);
+        launch_docs<HD, GEN, 1, 1, false, true>(a, s);
+    else if (HD <= 128 && p.NW == 1)
+        launch_docs<HD <= 128 ? HD : 64, GEN, 1, 1, false, false>(a, s);
     else
-        launch_docs<HD, GEN, NW, MINW, NS, AHEAD, false>(a, s);
+        launch_docs<HD, GEN, 4, MINW, AHEAD, false>(a, s);
 }
 
 int check_docs(int n, int rows_q, int rows_k, int Hq, int Hkv, int hd, int max_rows) {
@@ -745,7 +743,7 @@ extern "C" int mme_attention_docs(const void* q, long ldq, const void* k, long l
                                   void* stream) {
     if (int rc = check_docs(n, rows_q, rows_k, Hq, Hkv, hd, max_rows)) return rc;
     MME_REQUIRE(scale > 0.f && scale < INFINITY, "mme_attention_docs: scale must be positive and finite");
-    MME_REQUIRE(softcap >= 0.f && softcap < INFINITY, "mme_attention_docs: softcap must be 0 (none) or positive and finite");
+    MME_REQUIRE(softcap == 0.f || (softcap >= 1e-3f && softcap <= 1e3f), "mme_attention_docs: softcap must be 0 (none) or from 1e-3 to 1e3");
     MME_REQUIRE(causal || !prefix, "mme_attention_docs: a prefix goes with the causal mask");
     if (n == 0 || rows_q == 0) return MME_OK;
     MME_REQUIRE(q && out && q_offsets && k_offsets && (rows_k == 0 || (k && v)), "mme_attention_docs: null pointer");
@@ -759,7 +757,7 @@ extern "C" int mme_attention_docs(const void* q, long ldq, const void* k, long l
     const int mr = max_rows < rows_q ? max_rows : rows_q;
     if (mr == 0) return MME_OK;
     const Plan p = make_plan(n, rows_q, rows_k, Hkv, Hq / Hkv, hd, mr);
-    MME_REQUIRE(p.nslots >= 0 && (long)rows_q * (Hq / Hkv) < (1L << 31) - 512 && (long)n * Hkv * p.part_rows < (1L << 31),
+    MME_REQUIRE(p.nslots >= 0 && (long)rows_q * (Hq / Hkv) < (1L << 31) - 512 && rows_k < 0x7fff0000 && (long)n * Hkv * p.part_rows < (1L << 31),
                 "mme_attention_docs: too many rows");
     MME_REQUIRE(p.ws == 0 || (workspace && ws_bytes >= p.ws && ((uintptr_t)workspace & 15) == 0),
                 "mme_attention_docs: workspace of %zu bytes, %zu needed", ws_bytes, p.ws);
@@ -768,24 +766,24 @@ extern "C" int mme_attention_docs(const void* q, long ldq, const void* k, long l
     a.qoff = q_offsets, a.koff = k_offsets, a.prefix = prefix, a.slopes = slopes, a.part = (float*)workspace, a.stat = a.part + p.stat;
     a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldo = ldo, a.nslots = p.nslots;
     a.n = n, a.rows_q = rows_q, a.rows_k = rows_k, a.Hkv = Hkv, a.group = Hq / Hkv, a.hd = hd;
-    a.sorted = !p.split && n > 1 && n <= 63 && (long)p.nslots * Hkv >= SORTED, a.max_rows = mr, a.causal = causal ? 1 : 0, a.per_log2 = p.per_log2, a.part_rows = p.part_rows;
+    a.sorted = !p.split && n > 1 && n <= 63 && (long)p.nslots * Hkv >= 512, a.max_rows = mr, a.causal = causal ? 1 : 0, a.per = p.per, a.part_rows = p.part_rows, a.row_blocks = p.row_blocks;
     a.scale_log2 = scale * LOG2E;
     a.cap_log2 = softcap * LOG2E;
     a.cap_in = softcap != 0.f ? 2.0f * a.scale_log2 / softcap : 0.f;
     hipStream_t s = as_stream(stream);
     switch (hd) {
-        case 64: launch_width<64, false, NW64, MW64, NS64, AH64>(a, p, s); break;
-        case 72: launch_width<72, false, NW72, MW72, NS72, AH72>(a, p, s); break;
-        case 80: launch_width<80, false, NW72, MW72, NS72, AH72>(a, p, s); break;
-        case 128: launch_width<128, false, NW128, MW128, NS128, AH128>(a, p, s); break;
-        case 256: launch_width<256, false, NW256, MW256, NS256, AH256>(a, p, s); break;
+        case 64: launch_width<64, false, 3, false>(a, p, s); break;
+        case 72: launch_width<72, false, 3, false>(a, p, s); break;
+        case 80: launch_width<80, false, 3, false>(a, p, s); break;
+        case 128: launch_width<128, false, 2, true>(a, p, s); break;
+        case 256: launch_width<256, false, 2, false>(a, p, s); break;
         default:
             if (hd < 64)
-                launch_width<64, true, NW64, 2, 2, false>(a, p, s);
+                launch_width<64, true, 3, false>(a, p, s);
             else if (hd < 128)
-                launch_width<128, true, NW128, 2, 2, false>(a, p, s);
+                launch_width<128, true, 2, false>(a, p, s);
             else
-                launch_width<256, true, NW256, NW256 / 4, 2, false>(a, p, s);
+                launch_width<256, true, 1, false>(a, p, s);
     }
     if (p.split) {
         if (int rc = mme_check_launch("mme_attention_docs")) return rc;

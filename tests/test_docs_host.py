@@ -1,0 +1,106 @@
+"""Packed documents on the host: workspace sizes, refusals of the C entries (checked before any launch), frequencies
+and the oracle itself (no GPU)."""
+import numpy as np
+import pytest
+import torch
+
+from mme import _lib, ops
+from oracle import docs as oracle
+
+
+def ws(n, rows, keys, Hq, Hkv, hd, max_rows):
+    return _lib.query("mme_attention_docs_workspace_bytes", n, rows, keys, Hq, Hkv, hd, max_rows)
+
+
+@pytest.mark.parametrize("args", [(0, 0, 0, 1, 1, 64, 0), (1, 0, 5000, 8, 1, 256, 0), (3, 10, 0, 8, 1, 256, 10),
+                                  (3, 10, 90000, 8, 1, 256, 0), (1, 2147483647, 2147418111, 1, 1, 8, 2147483647),
+                                  (2147483646, 1, 1, 65535, 65535, 256, 1), (100000, 100000, 2000000000, 64, 64, 128, 1)])
+def test_workspace_sizes_of_the_ends(args):
+    assert ws(*args) >= 0
+
+
+def test_workspace_is_for_few_rows_and_many_keys_alone():
+    assert ws(1, 1, 60000, 8, 1, 256, 1) > 0
+    assert ws(1, 60000, 60000, 8, 1, 256, 60000) == 0        # as many rows as keys
+    assert ws(64, 64, 64 * 100, 8, 1, 256, 1) == 0           # short documents
+    assert ws(1, 1, 60000, 8, 1, 12, 1) == 0                 # refused
+    # chunks of at least a tile for two rounds of workgroups: some ten thousand partial rows at most
+    assert ws(64, 64, 64 * 100000, 32, 8, 128, 1) < 64 << 20
+
+
+DOCS = dict(q=16, ldq=512, k=16, ldk=128, v=16, ldv=128, out=16, ldo=512, q_off=16, k_off=16, n=2, rows_q=8, rows_k=8, Hq=8,
+            Hkv=2, hd=64, max_rows=8, causal=1, prefix=None, softcap=0.0, slopes=None, scale=0.1, ws=None, ws_bytes=0)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(hd=12), "head_dim 12"), (dict(hd=136), "head_dim 136"), (dict(hd=512), "head_dim 512"), (dict(Hkv=3), "8 heads over 3"),
+    (dict(Hkv=0), "over 0"), (dict(n=-1), "bad shape"), (dict(max_rows=-1), "bad shape"), (dict(scale=0.0), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(softcap=-1.0), "softcap"), (dict(softcap=2e3), "softcap"),
+    (dict(softcap=float("nan")), "softcap"), (dict(causal=0, prefix=16), "prefix"), (dict(q=None), "null"),
+    (dict(v=None), "null"), (dict(k_off=None), "null"), (dict(ldq=511), "leading"), (dict(ldk=127), "leading"),
+    (dict(ldo=504), "leading"), (dict(ldv=1 << 24), "2\\^24"), (dict(q=8), "misaligned"), (dict(out=24), "misaligned"),
+    (dict(q_off=18), "misaligned"), (dict(rows_k=2147483647), "too many"),
+    (dict(n=1, rows_q=1, rows_k=60000, max_rows=1), "workspace"),
+    (dict(n=1, rows_q=1, rows_k=60000, max_rows=1, ws=16, ws_bytes=100), "workspace"),
+    (dict(n=1, rows_q=1, rows_k=60000, max_rows=1, ws=8, ws_bytes=1 << 40), "workspace")])
+def test_attention_docs_refusals(change, match):
+    with pytest.raises(_lib.MMEError, match=match):
+        _lib.call("mme_attention_docs", *{**DOCS, **change}.values(), None)
+
+
+ROPE = dict(x=16, ldx=128, y=16, ldy=128, rows=4, nheads=2, hd=64, pairs=32, pos=16, ldp=4, naxes=1, freqs=16, axes=16,
+            adjacent=0, inverse=0)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(pairs=33), "33 pairs"), (dict(pairs=0), "0 pairs"), (dict(nheads=0), "bad shape"), (dict(rows=-1), "bad shape"),
+    (dict(naxes=0), "bad shape"), (dict(ldx=127), "leading"), (dict(ldp=3), "leading"), (dict(ldy=130), "in place"),
+    (dict(x=None), "null"), (dict(freqs=None), "null"), (dict(freqs=12), "misaligned"), (dict(x=17), "misaligned"),
+    (dict(nheads=65535, hd=4096, ldx=1 << 40, ldy=1 << 40), "rows of")])
+def test_rope_axes_refusals(change, match):
+    with pytest.raises(_lib.MMEError, match=match):
+        _lib.call("mme_rope_axes", *{**ROPE, **change}.values(), None)
+
+
+def test_no_work_is_no_error():
+    _lib.call("mme_rope_axes", *{**ROPE, "rows": 0, "x": None, "y": None, "pos": None}.values(), None)
+    for change in (dict(n=0), dict(rows_q=0, q=None), dict(max_rows=0)):
+        _lib.call("mme_attention_docs", *{**DOCS, **change}.values(), None)
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 128, dtype=torch.bfloat16)
+    off = torch.tensor([0, 4], dtype=torch.int32)
+    f, a = ops.rope_axes_freqs((32,), 1e4, device="cpu")
+    with pytest.raises(ValueError, match="CPU tensor"):
+        ops.attention_docs(x, x, x, off, 2, 2)
+    with pytest.raises(ValueError, match="CPU tensor"):
+        ops.rope_axes(x, torch.zeros(1, 4, dtype=torch.int32), f, a, 2)
+
+
+def test_rope_axes_freqs():
+    f, a = ops.rope_axes_freqs((2, 3), 100.0, device="cpu")
+    assert a.tolist() == [0, 0, 1, 1, 1] and a.dtype == torch.int32 and f.dtype == torch.float64
+    assert torch.allclose(f, 100.0 ** (-torch.arange(5).double() / 5), rtol=1e-15)
+    f, a = ops.rope_axes_freqs((2, 0, 3), 100.0, in_turns=True, per_axis=True, device="cpu")
+    assert a.tolist() == [0, 2, 0, 2, 2]
+    assert torch.allclose(f, torch.tensor([1.0, 1.0, 0.1, 100.0 ** (-1 / 3), 100.0 ** (-2 / 3)], dtype=torch.float64), rtol=1e-15)
+
+
+def test_the_oracle_against_torch():
+    """One document without a mask is torch's softmax attention in float64; the rotation is a complex product."""
+    r = np.random.RandomState(0)
+    q, k, v = r.randn(7, 32), r.randn(9, 16), r.randn(9, 16)
+    o, _, _ = oracle.attention_docs(q, k, v, [0, 7], 4, 2, key_offsets=[0, 9])
+    t = lambda x, h: torch.from_numpy(x).view(x.shape[0], h, 8).transpose(0, 1)  # noqa: E731
+    kk, vv = t(k, 2).repeat_interleave(2, 0), t(v, 2).repeat_interleave(2, 0)
+    want = torch.softmax(t(q, 4) @ kk.transpose(1, 2) / 8 ** 0.5, -1) @ vv
+    assert np.allclose(o, want.transpose(0, 1).reshape(7, 32).numpy(), atol=1e-14)
+    o, _, _ = oracle.attention_docs(q, k, v, [0, 7], 4, 2, key_offsets=[0, 9], causal=True)
+    seen = torch.arange(9)[None, :] <= torch.arange(7)[:, None] + 2
+    s = (t(q, 4) @ kk.transpose(1, 2) / 8 ** 0.5).masked_fill(~seen, -float("inf"))
+    assert np.allclose(o, (torch.softmax(s, -1) @ vv).transpose(0, 1).reshape(7, 32).numpy(), atol=1e-14)
+    x = r.randn(3, 8)
+    y, _ = oracle.rope_axes(x, np.array([[1, 2, 3], [5, 7, 9]]), [1.0, 0.5], [0, 1], 2, 4, adjacent=True)
+    z = (x[:, 0::2] + 1j * x[:, 1::2]) * np.exp(1j * np.array([[1.0, 2.5], [2.0, 3.5], [3.0, 4.5]]))[:, [0, 1, 0, 1]]
+    assert np.allclose(y[:, 0::2], z.real, atol=1e-14) and np.allclose(y[:, 1::2], z.imag, atol=1e-14)

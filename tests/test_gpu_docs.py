@@ -208,6 +208,33 @@ def test_docs_few_queries(cuda, heads, kv_heads, hd, klens, qlen, full):
     check_docs(ops.attention_docs(q, k, v, off, heads, kv_heads, **kw), q, k, v, off, heads, kv_heads, **kw)
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd", [(4, 1, 40), (3, 1, 96), (2, 2, 144), (8, 1, 256), (4, 4, 72), (2, 1, 80),
+                                               (8, 2, 128)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_docs_several_blocks_of_rows_against_split_keys(cuda, heads, kv_heads, hd, causal):
+    from mme import ops
+    g = gen(hd * 3 + heads)
+    qlens, klens = (30, 1, 17), (900, 1300, 20)
+    q, k, v = make(g, sum(qlens), sum(klens), heads, kv_heads, hd, cuda)
+    off, koff = cuts(qlens).to(cuda), cuts(klens).to(cuda)
+    kw = dict(key_offsets=koff, max_rows=30, causal=causal)
+    check_docs(ops.attention_docs(q, k, v, off, heads, kv_heads, **kw), q, k, v, off, heads, kv_heads, **kw)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_docs_masked_values_in_split_keys(cuda, value):
+    """The later of two query rows sees a key whose v is not finite, the earlier one does not."""
+    from mme import ops
+    g = gen(23)
+    q, k, v = make(g, 4, 1600, 4, 1, 128, cuda)
+    off, koff = cuts((2, 2)).to(cuda), cuts((800, 800)).to(cuda)
+    v[799] = value
+    kw = dict(key_offsets=koff, max_rows=2, causal=True)
+    got = ops.attention_docs(q, k, v, off, 4, 1, **kw)
+    check_docs(got, q, k, v, off, 4, 1, rows=np.array([True, False, True, True]), **kw)
+    assert not torch.isfinite(got[1].float()).any()
+
+
 def test_docs_rows_that_see_nothing_are_zero(cuda):
     from mme import ops
     g = gen(11)
@@ -359,6 +386,7 @@ def test_docs_refusals(cuda):
             bad()
     for bad in (lambda: f(q, k, k, off, 4, 2, scale=0.0), lambda: f(q, k, k, off, 4, 2, scale=float("inf")),
                 lambda: f(q, k, k, off, 4, 2, scale=float("nan")), lambda: f(q, k, k, off, 4, 2, softcap=-1.0),
+                lambda: f(q, k, k, off, 4, 2, softcap=1e-4), lambda: f(q, k, k, off, 4, 2, softcap=1e4),
                 lambda: f(q, k, k, off, 4, 2, softcap=float("nan")),
                 lambda: f(q[:, :4 * 12], k[:, :2 * 12], k[:, :2 * 12], off, 4, 2),           # head dim 12
                 lambda: f(q[:, 4:4 + 4 * 56], k[:, :2 * 56], k[:, :2 * 56], off, 4, 2)):     # 8-byte base
