@@ -96,8 +96,10 @@ __device__ __forceinline__ Doc find_doc(const DocsArgs& a, int slot) {
     const int pr = a.prefix ? a.prefix[min(i, a.n - 1)] : 0;
     int fs = first_slot(SPLIT ? ko : qo, i, mul, a.per), l;
     if (SORT && a.sorted) {
-        const int kl = lane < a.n ? __shfl_down(ko, 1, 64) - ko : -1;
-        const int parts = lane < a.n ? (min(max(__shfl_down(qo, 1, 64) - qo, 0), a.max_rows) * mul + a.per - 1) / a.per : 0;
+        // every lane takes part in the exchange: document n - 1 needs lane n's offsets
+        const int ql = __shfl_down(qo, 1, 64) - qo, kd = __shfl_down(ko, 1, 64) - ko;
+        const int kl = lane < a.n ? max(kd, 0) : -1;
+        const int parts = lane < a.n ? (min(max(ql, 0), a.max_rows) * mul + a.per - 1) / a.per : 0;
         fs = 0;  // the slots of the documents before this lane's
         for (int j = 0; j < a.n; ++j) {
             const int kj = __builtin_amdgcn_readlane(kl, j), pj = __builtin_amdgcn_readlane(parts, j);
@@ -120,10 +122,10 @@ __device__ __forceinline__ Doc find_doc(const DocsArgs& a, int slot) {
     return r;
 }
 
-// HD: the head dim, or with GEN the least of 64, 128, 256 that holds it
-template <int HD, bool GEN>
+// HD: the head dim, or with GEN the least of 64, 128, 256 that holds it. KT: keys a tile, 64, or 32 where head dim 256
+// keeps its registers and LDS at half, and for short documents.
+template <int HD, bool GEN, int KT>
 struct Tile {
-    static constexpr int KT = HD > 128 ? 32 : 64;   // keys a tile: head dim 256 keeps its registers and LDS at half
     static constexpr int KB = KT / 32;
     static constexpr int NKS = (HD + 15) / 16;        // k-steps of Q K^T
     static constexpr int NDB = (HD + 31) / 32;        // 32-column blocks of O^T
@@ -142,7 +144,7 @@ struct Tile {
     // the 16 rows of a K read, into banks of their own.
     static constexpr bool ONES = HD == 72 || HD == 80;
     static constexpr int KP = ONES ? 9 + (HD == 80 ? 2 : 0) : HD / 8, VP = ONES ? 12 : HD / 8;  // chunks a row (not GEN)
-    static constexpr int NPK = KT * KP / 64, NPV = KT * VP / 64;                                // pieces of K, and of V
+    static constexpr int NPK = (KT * KP + 63) / 64, NPV = (KT * VP + 63) / 64;                  // pieces of K, and of V
     static constexpr int VOFF = NPK * (1024 + KGAP);
     static constexpr int BYTES = VOFF + NPV * (1024 + VGAP);
     // where row `row` of K or V begins (rows of a piece are contiguous); nch: chunks a row
@@ -199,8 +201,9 @@ __device__ __forceinline__ void row_alone(const DocsArgs& a, const Doc& D, int g
 // AHEAD: the next tile's scores are formed beside this one's weights
 template <int HD, bool GEN, int NW, int MINW, bool AHEAD, bool SPLIT, int MODE>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW))) void attn_docs_kernel(DocsArgs a) {
-    using T = Tile<HD, GEN>;
-    constexpr int KT = T::KT, KB = T::KB, NKS = T::NKS, NDB = T::NDB, QB = NW * 32;
+    constexpr int KT = HD > 128 || (NW == 1 && !SPLIT) ? 32 : 64;
+    using T = Tile<HD, GEN, KT>;
+    constexpr int KB = T::KB, NKS = T::NKS, NDB = T::NDB, QB = NW * 32;
     constexpr bool HALF = GEN || HD % 16 != 0;  // the last k-step may reach past the head dim
     constexpr int ZERO = 2 * T::BYTES;           // 16 zero bytes for it
     __shared__ __attribute__((aligned(16))) char lds[2 * T::BYTES + (HALF ? 16 : 0)];
@@ -261,7 +264,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     const char* vbase = (const char*)(a.v + (D.k0 + (long)key_lo) * a.ldv + (long)kvh * a.hd);
     // a tile of K (V) is kp (vp) * KT / 64 pieces; piece p: LDS chunks 64 p .. + 63, chunk c of row (64 p + lane) / kp.
     // A lane's places in them are the same in every tile but one that reaches past the document.
-    const int npk = GEN ? nch * KT / 64 : T::NPK, npv = GEN ? nch * KT / 64 : T::NPV;
+    const int npk = GEN ? (nch * KT + 63) / 64 : T::NPK, npv = GEN ? npk : T::NPV;
     if (T::ONES)
         for (int i = tid; i < 2 * KT; i += NW * 64)
             *reinterpret_cast<u16x8*>(lds + i / KT * T::BYTES + T::VOFF + (i % KT * T::VP + HD / 8) * 16) =
@@ -274,13 +277,16 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
                    : (unsigned)min(row, most) * (unsigned)(2 * a.ldk) + (ch ^ T::kx(row)) * 16;
     };
     constexpr int PK = (T::NPK + NW - 1) / NW, PV = (T::NPV + NW - 1) / NW;
-    constexpr bool KFULL = GEN || T::KP == HD / 8, VFULL = GEN || T::VP == HD / 8;  // no chunk to leave out
+    // no chunk to leave out: behind a row's data, or behind the tile in a last piece that is half one
+    constexpr bool KFULL = GEN ? KT == 64 : T::KP == HD / 8 && KT * T::KP % 64 == 0;
+    constexpr bool VFULL = GEN ? KT == 64 : T::VP == HD / 8 && KT * T::VP % 64 == 0;
+    auto has = [&](bool isV, int i) __attribute__((always_inline)) { return chunk_of(isV, i) < nch && row_of(isV, i) < KT; };
     unsigned atk[PK], atv[PV];
     bool dok[PK], dov[PV];
 #pragma unroll
-    for (int i = 0; i < PK; ++i) atk[i] = place(false, i, KT), dok[i] = chunk_of(false, i) < nch;
+    for (int i = 0; i < PK; ++i) atk[i] = place(false, i, KT), dok[i] = has(false, i);
 #pragma unroll
-    for (int i = 0; i < PV; ++i) atv[i] = place(true, i, KT), dov[i] = chunk_of(true, i) < nch;
+    for (int i = 0; i < PV; ++i) atv[i] = place(true, i, KT), dov[i] = has(true, i);
     auto issue = [&](auto v_c, int t, unsigned slot) __attribute__((always_inline)) {
         constexpr bool isV = decltype(v_c)::value;
         const char* base = isV ? vbase + (long)t * KT * 2 * a.ldv : kbase + (long)t * KT * 2 * a.ldk;
@@ -294,7 +300,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
         } else {
 #pragma unroll 1
             for (int i = 0; wave + NW * i < np; ++i)
-                if ((isV ? VFULL : KFULL) || chunk_of(isV, i) < nch) dma16(base, place(isV, i, most), to + (wave + NW * i) * pitch);
+                if ((isV ? VFULL : KFULL) || has(isV, i)) dma16(base, place(isV, i, most), to + (wave + NW * i) * pitch);
         }
     };
     if (nkt > 0) issue(std::false_type{}, 0, 0);
@@ -670,10 +676,11 @@ Plan make_plan(int n, int rows_q, int rows_k, int Hkv, int group, int hd, int ma
     Plan p{};
     if (n == 0 || max_rows == 0) return p;
     const long flat = (long)rows_q * group, keys = (long)rows_k / n;
-    // One wave a workgroup where documents fill no more than one and there are workgroups enough; else four, also
-    // where three of them only help to copy. 12 000 rows in documents of 16 / 32 / 48 rows, 12 heads of 64: one wave
-    // 42 / 26 / 29 us, four 51 / 29 / 23; one key head of 256 (32 flat rows) 79 and 46.
-    p.NW = flat / n <= 32 && hd <= 128 && (flat / 32 + n) * Hkv >= 512 ? 1 : 4;
+    // One wave a workgroup (and tiles of 32 keys, so that many fit a CU) for short documents, where there are workgroups
+    // enough; else four, which share the tiles and the copying. 12 000 rows in documents of 48 / 128 / 256 rows, 12
+    // heads of 64: one wave 20 / 22 / 28 us, four 24 / 25 / 31; documents of 12 / 32 / 64 rows, 4 heads of 128 to each of
+    // 8 key heads, 92 / 72 / 86 and 121 / 98 / 62.
+    p.NW = hd <= 128 && (flat / n <= 32 || (flat / n <= 128 && keys <= 256)) && (flat / 32 + n) * Hkv >= 512 ? 1 : 4;
     p.per = p.NW * 32;
     p.row_blocks = 1;
     long nslots = flat / p.per + n;
@@ -716,7 +723,7 @@ void launch_width(const DocsArgs& a, const Plan& p, hipStream_t s) {
     if (p.split)
         launch_docs<HD, GEN, 1, 1, false, true>(a, s);
     else if (HD <= 128 && p.NW == 1)
-        launch_docs<HD <= 128 ? HD : 64, GEN, 1, 1, false, false>(a, s);
+        launch_docs<HD <= 128 ? HD : 64, GEN, 1, HD <= 80 ? 2 : 1, false, false>(a, s);
     else
         launch_docs<HD, GEN, 4, MINW, AHEAD, false>(a, s);
 }

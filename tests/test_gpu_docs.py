@@ -235,6 +235,62 @@ def test_docs_masked_values_in_split_keys(cuda, value):
     assert not torch.isfinite(got[1].float()).any()
 
 
+LARGE = [
+    # document lengths, heads, kv_heads, hd, what else: enough workgroups that the longest documents go first
+    ((700, 64, 1500, 0, 333, 1, 64, 900), 16, 16, 72, {}),
+    ((1040, 1060, 1031), 8, 1, 256, dict(causal=True, prefix=True, softcap=50.0)),
+    ((2500, 3, 1700), 16, 8, 128, dict(causal=True)),
+    ((5, 40, 1900, 77, 800), 24, 24, 64, dict(slopes=True)),
+    ((300,) * 40, 5, 5, 96, dict(causal=True, slopes=True, softcap=30.0)),
+    ((129,) * 63, 12, 4, 80, dict(causal=True)),
+    ((129,) * 64, 12, 4, 80, dict(causal=True)),
+    ((2100, 1700, 1), 6, 2, 240, {}),
+]
+
+
+@pytest.mark.parametrize("lens,heads,kv_heads,hd,what", LARGE, ids=lambda v: str(v)[:20])
+def test_docs_large(cuda, lens, heads, kv_heads, hd, what):
+    """Whole outputs of large calls against float64 products on the device, a document and a head at a time."""
+    from mme import ops
+    g = gen(sum(lens) + hd)
+    rows = sum(lens)
+    q, k, v = make(g, rows, rows, heads, kv_heads, hd, cuda)
+    off = cuts(lens).to(cuda)
+    kw = dict(causal=what.get("causal", False), softcap=what.get("softcap", 0.0))
+    if "prefix" in what:
+        kw["prefix"] = torch.tensor([n * 3 // 4 for n in lens], dtype=torch.int32, device=cuda)
+    if "slopes" in what:
+        kw["slopes"] = (2.0 ** -torch.arange(1, heads + 1).float()).to(cuda)
+    out = torch.full((rows, heads * hd), float("nan"), dtype=BF16, device=cuda)
+    got = ops.attention_docs(q, k, v, off, heads, kv_heads, out=out, **kw).double()
+    row = 0
+    for d, n in enumerate(lens):
+        at = torch.arange(n, device=cuda)
+        last = at + 1
+        if "prefix" in kw:
+            last = torch.maximum(last, kw["prefix"][d].long())
+        for h in range(heads if n else 0):
+            j = h * kv_heads // heads
+            qq, kk, vv = (t[row:row + n, i * hd:(i + 1) * hd].double().contiguous() for t, i in ((q, h), (k, j), (v, j)))
+            s = qq @ kk.t().contiguous() * hd ** -0.5
+            big = qq.abs() @ kk.abs().t().contiguous() * hd ** -0.5
+            if kw["softcap"]:
+                s = kw["softcap"] * torch.tanh(s / kw["softcap"])
+            if "slopes" in kw:
+                bias = kw["slopes"][h].double() * (at[:, None] - at[None, :]).abs()
+                s, big = s - bias, big + bias
+            if kw["causal"]:
+                s = s.masked_fill(at[None, :] >= last[:, None], -float("inf"))
+            w = torch.softmax(s, -1)
+            want, spread = w @ vv, w @ vv.abs()
+            # as in check_docs
+            delta = (hd + 4) * 2.0 ** -24 * big.amax(1, keepdim=True) + 3 * kw["softcap"] * 2.0 ** -23 + 2.0 ** -20
+            tol = HALF * (spread + 2 * want.abs()) + 2 * (spread + want.abs()) * delta + n * 2.0 ** -24 * spread
+            bad = ~((got[row:row + n, h * hd:(h + 1) * hd] - want).abs() <= tol)
+            assert not bad.any(), (d, h, bad.nonzero()[:5])
+        row += n
+
+
 def test_docs_rows_that_see_nothing_are_zero(cuda):
     from mme import ops
     g = gen(11)
