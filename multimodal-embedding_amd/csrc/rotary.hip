@@ -210,7 +210,7 @@ extern "C" int mme_rope_axes(const void* x, long ldx, void* y, long ldy, int row
     MME_REQUIRE(rows >= 0 && nheads > 0 && nheads <= 65535 && naxes > 0, "mme_rope_axes: bad shape");
     MME_REQUIRE(pairs > 0 && hd > 0 && 2L * pairs <= hd, "mme_rope_axes: %d pairs do not fit a head of %d", pairs, hd);
     MME_REQUIRE((long)nheads * hd < (1L << 24), "mme_rope_axes: rows of %ld elements", (long)nheads * hd);
-    MME_REQUIRE(ldx >= (long)nheads * hd && ldy >= (long)nheads * hd && ld_pos >= rows, "mme_rope_axes: bad leading dims");
+    MME_REQUIRE(ldx >= (long)nheads * hd && ldy >= (long)nheads * hd && ld_pos >= 0, "mme_rope_axes: bad leading dims");
     if (rows == 0) return MME_OK;
     MME_REQUIRE(x && y && positions && freqs && axes, "mme_rope_axes: null pointer");
     MME_REQUIRE(x != y || ldx == ldy, "mme_rope_axes: in place with two leading dims");

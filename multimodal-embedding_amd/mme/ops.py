@@ -467,7 +467,8 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axe
     """Rotary positions with several axes (mme_rope_axes): pair i of heads [0, nheads) of each row turns by
     positions[axes[i], row] * freqs[i].
 
-    x: bf16 [rows, >= nheads * hd] (hd defaults to x.shape[1] // nheads); positions: int32 [naxes, rows]; freqs:
+    x: bf16 [rows, >= nheads * hd] (hd defaults to x.shape[1] // nheads); positions: int32 [naxes, rows], rows of it
+    contiguous (one row expanded to all axes will do); freqs:
     float64 [pairs]; axes: int32 [pairs] (rope_axes_freqs makes both). The pair is elements (i, i + pairs) of a head,
     or (2i, 2i + 1) with adjacent; elements from 2 * pairs on are copied. inverse turns back: the gradient with
     respect to x is this of the gradient with respect to the result. out: None for a new tensor, x itself for in
@@ -503,7 +504,7 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axe
         ldo = _rowmajor(out, "out")
     ev = KernelTimer.begin()
     call("mme_rope_axes", x.data_ptr(), ldx, out.data_ptr(), ldo, rows, nheads, hd, pairs, positions.data_ptr(),
-         ldp if ldp > rows else rows, naxes, freqs.data_ptr(), axes.data_ptr(), adjacent, inverse, _raw_stream(dev))
+         ldp, naxes, freqs.data_ptr(), axes.data_ptr(), adjacent, inverse, _raw_stream(dev))
     if ev is not None:
         KernelTimer.end(ev, "rope_axes", 0.0, 4.0 * rows * nheads * hd)
     return out
@@ -547,20 +548,24 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: t
     key_offsets = offsets if key_offsets is None else key_offsets
     dev = q.get_device()
     if dev < 0 or not dev == k.get_device() == v.get_device() == offsets.get_device() == key_offsets.get_device() \
-            or any(t is not None and t.get_device() != dev for t in (prefix, slopes, out)):
+            or (prefix is not None and prefix.get_device() != dev) \
+            or (slopes is not None and slopes.get_device() != dev) or (out is not None and out.get_device() != dev):
         _elsewhere("attention_docs", q, k, v, offsets, key_offsets, prefix, slopes, out)
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return attention_docs(q, k, v, offsets, heads, kv_heads, key_offsets=key_offsets, max_rows=max_rows,
                                   causal=causal, prefix=prefix, softcap=softcap, slopes=slopes, scale=scale, out=out)
-    ldq, ldk, ldv = _rowmajor(q, "q"), _rowmajor(k, "k"), _rowmajor(v, "v")
-    (rows, width), keys, n = q.shape, k.shape[0], offsets.numel() - 1
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    if not len(sq) == len(sk) == len(sv) == 2 or not sq[1] == sk[1] == sv[1] == 1:
+        for t, name in ((q, "q"), (k, "k"), (v, "v")):
+            _rowmajor(t, name)
+    (rows, width), (keys, kwidth), n = q.shape, k.shape, offsets.numel() - 1
     if heads < 1 or kv_heads < 1 or heads % kv_heads or width % heads:
         raise ValueError(f"attention_docs: {heads} heads over {kv_heads} key heads in rows of {width}")
     hd = width // heads
     if q.dtype is not BF16 or k.dtype is not BF16 or v.dtype is not BF16:
         raise ValueError("attention_docs: q, k and v must be bf16")
-    if k.shape != v.shape or k.shape[1] != kv_heads * hd:
+    if kwidth != kv_heads * hd or k.shape != v.shape:
         raise ValueError(f"attention_docs: k {tuple(k.shape)} and v {tuple(v.shape)} must be [keys, {kv_heads * hd}]")
     for t in (offsets,) if key_offsets is offsets else (offsets, key_offsets):
         if n < 0 or t.numel() != n + 1 or t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
@@ -583,11 +588,13 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: t
         raise ValueError(f"attention_docs: out must be bf16 [{rows}, >= {width}]")
     else:
         ldo = _rowmajor(out, "out")
-    wsb = query("mme_attention_docs_workspace_bytes", n, rows, keys, heads, kv_heads, hd, max_rows)
-    # a workspace of the call's own: calls on two streams, or in two captured graphs, share none
-    ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
+    ws, wsb = None, 0
+    if max_rows * heads <= 256 * kv_heads and keys * hd >= 40960 * n:  # none is needed otherwise (mme.h)
+        wsb = query("mme_attention_docs_workspace_bytes", n, rows, keys, heads, kv_heads, hd, max_rows)
+        # a workspace of the call's own: calls on two streams, or in two captured graphs, share none
+        ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
     ev = KernelTimer.begin()
-    call("mme_attention_docs", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo,
+    call("mme_attention_docs", q.data_ptr(), sq[0], k.data_ptr(), sk[0], v.data_ptr(), sv[0], out.data_ptr(), ldo,
          offsets.data_ptr(), key_offsets.data_ptr(), n, rows, keys, heads, kv_heads, hd, max_rows, bool(causal),
          _ptr(prefix), softcap, _ptr(slopes), hd ** -0.5 if scale is None else scale, _ptr(ws), wsb, _raw_stream(dev))
     if ev is not None:

@@ -28,6 +28,20 @@ def test_workspace_is_for_few_rows_and_many_keys_alone():
     assert ws(64, 64, 64 * 100000, 32, 8, 128, 1) < 64 << 20
 
 
+def test_workspace_is_none_where_the_header_says_so():
+    r = np.random.RandomState(3)
+    some = 0
+    for _ in range(3000):
+        n, hkv, group = int(r.randint(1, 300)), int(r.choice([1, 2, 8, 16])), int(r.choice([1, 2, 4, 8]))
+        hd = int(r.choice([8, 64, 72, 80, 128, 192, 256]))
+        keys, rows = int(n * 2 ** r.uniform(0, 16)), int(n * 2 ** r.uniform(0, 8))
+        most = int(2 ** r.uniform(0, 10))
+        size = ws(n, rows, keys, hkv * group, hkv, hd, most)
+        some += size > 0
+        assert size == 0 or (min(most, rows) * group <= 256 and keys * hd >= 40960 * n)
+    assert some > 100
+
+
 DOCS = dict(q=16, ldq=512, k=16, ldk=128, v=16, ldv=128, out=16, ldo=512, q_off=16, k_off=16, n=2, rows_q=8, rows_k=8, Hq=8,
             Hkv=2, hd=64, max_rows=8, causal=1, prefix=None, softcap=0.0, slopes=None, scale=0.1, ws=None, ws_bytes=0)
 
@@ -54,7 +68,7 @@ ROPE = dict(x=16, ldx=128, y=16, ldy=128, rows=4, nheads=2, hd=64, pairs=32, pos
 
 @pytest.mark.parametrize("change,match", [
     (dict(pairs=33), "33 pairs"), (dict(pairs=0), "0 pairs"), (dict(nheads=0), "bad shape"), (dict(rows=-1), "bad shape"),
-    (dict(naxes=0), "bad shape"), (dict(ldx=127), "leading"), (dict(ldp=3), "leading"), (dict(ldy=130), "in place"),
+    (dict(naxes=0), "bad shape"), (dict(ldx=127), "leading"), (dict(ldp=-1), "leading"), (dict(ldy=130), "in place"),
     (dict(x=None), "null"), (dict(freqs=None), "null"), (dict(freqs=12), "misaligned"), (dict(x=17), "misaligned"),
     (dict(nheads=65535, hd=4096, ldx=1 << 40, ldy=1 << 40), "rows of")])
 def test_rope_axes_refusals(change, match):

@@ -81,6 +81,9 @@ def test_rope_axes_strides_and_what_it_leaves(cuda):
     f1, a1 = ops.rope_axes_freqs((32,), 1e4, device=cuda)
     p1 = torch.arange(20, dtype=torch.int32, device=cuda)[None]
     check_rope(ops.rope_axes(odd, p1, f1, a1, 2, hd=64), odd.cpu(), p1.cpu(), f1.cpu(), a1.cpu(), 2, 64)
+    # one row of positions for all axes
+    f3, a3 = ops.rope_axes_freqs((10, 11, 11), 1e4, device=cuda)
+    assert torch.equal(ops.rope_axes(odd, p1.expand(3, 20), f3, a3, 2, hd=64), ops.rope_axes(odd, p1, f1, a1, 2, hd=64))
     # axes outside the positions are clamped, no rows are no work
     a2 = torch.full_like(a1, 5)
     assert torch.equal(ops.rope_axes(odd, p1, f1, a2, 2, hd=64), ops.rope_axes(odd, p1, f1, a1, 2, hd=64))
