@@ -365,6 +365,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
                 if (!GEN || 2 * ks < nch) z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfrag(so, kb, ks), qf[ks], z, 0, 0, 0);
             sc[kb] = z;
         }
+        if (!GEN) {  // reads four ahead of the products that take them
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int x = 0; x < KB * NKS - 4; ++x) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        }
     };
     // register e of block kb scores key key0 + 32 kb + (e & 3) + 8 (e >> 2) + 4 hh; CUT: some row may not see all keys
     auto score = [&](auto cut_c, f32x16(&sc)[KB], int t) __attribute__((always_inline)) {
@@ -454,6 +463,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
 #pragma unroll
             for (int db = 0; db < NDB; ++db)
                 o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfrag(so, i, db), pk[i], o[db], 0, 0, 0);
+        if (!GEN) {  // and three
+            __builtin_amdgcn_sched_group_barrier(0x100, 6, 1);
+#pragma unroll
+            for (int x = 0; x < 2 * KB * NDB - 3; ++x) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 3, 1);
+        }
     };
     // this wave's part of the next tile has landed and its LDS reads are done; then everybody's
     auto meet = [&]() __attribute__((always_inline)) {
