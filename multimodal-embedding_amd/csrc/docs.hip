@@ -220,14 +220,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
         const int bid = blockIdx.x, nwg = gridDim.x;
         const int xcd = bid & 7, loc = bid >> 3, q8 = nwg >> 3, r8 = nwg & 7;
         const int id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + loc;
-        if (OWN) {
+        if constexpr (OWN) {
             const int x = SPLIT ? id / a.row_blocks : id;  // split: the blocks of rows of one chunk side by side too
             rb = id - x * (SPLIT ? a.row_blocks : 1), slot = x / a.Hkv, kvh = x - slot * a.Hkv;
-        }
-        else if ((a.Hkv & 7) == 0)
+        } else if ((a.Hkv & 7) == 0) {
             slot = loc / (a.Hkv >> 3), kvh = xcd * (a.Hkv >> 3) + loc - slot * (a.Hkv >> 3);
-        else
+        } else {
             kvh = id / a.nslots, slot = id - kvh * a.nslots;
+        }
     }
     const Doc D = find_doc<SPLIT, !OWN>(a, slot);
     const int qlen = D.qlen, klen = D.klen;
@@ -603,6 +603,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
         }
     }
     if (__builtin_amdgcn_ballot_w64(found) == 0) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the rows' first stores come before their second
     for (int x = 0; x < 32; ++x) {
         if (!(bad >> x & 1)) continue;
         const int fx = f0 + wave * 32 + x, qx = fx / a.group, gx = kvh * a.group + fx - qx * a.group, px = qx + klen - qlen;

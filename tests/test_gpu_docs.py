@@ -81,6 +81,13 @@ def test_rope_axes_strides_and_what_it_leaves(cuda):
     f1, a1 = ops.rope_axes_freqs((32,), 1e4, device=cuda)
     p1 = torch.arange(20, dtype=torch.int32, device=cuda)[None]
     check_rope(ops.rope_axes(odd, p1, f1, a1, 2, hd=64), odd.cpu(), p1.cpu(), f1.cpu(), a1.cpu(), 2, 64)
+    # 4-byte alignment, both layouts, in and out of place
+    four = randn(g, 20, 2 * 64 + 2).to(cuda)[:, 2:]
+    for adjacent in (False, True):
+        want = ops.rope_axes(four, p1, f1, a1, 2, hd=64, adjacent=adjacent)
+        check_rope(want, four.cpu(), p1.cpu(), f1.cpu(), a1.cpu(), 2, 64, adjacent=adjacent)
+        inside = torch.empty(20, 130, dtype=BF16, device=cuda)[:, 2:].copy_(four)
+        assert torch.equal(ops.rope_axes(inside, p1, f1, a1, 2, hd=64, adjacent=adjacent, out=inside), want)
     # one row of positions for all axes
     f3, a3 = ops.rope_axes_freqs((10, 11, 11), 1e4, device=cuda)
     assert torch.equal(ops.rope_axes(odd, p1.expand(3, 20), f3, a3, 2, hd=64), ops.rope_axes(odd, p1, f1, a1, 2, hd=64))
@@ -88,6 +95,24 @@ def test_rope_axes_strides_and_what_it_leaves(cuda):
     a2 = torch.full_like(a1, 5)
     assert torch.equal(ops.rope_axes(odd, p1, f1, a2, 2, hd=64), ops.rope_axes(odd, p1, f1, a1, 2, hd=64))
     assert ops.rope_axes(odd[:0], p1[:, :0], f1, a1, 2, hd=64).shape == (0, 128)
+
+
+@pytest.mark.parametrize("heads,hd,sections,adjacent", [(9, 128, (20, 22, 22), False), (32, 72, (18, 18), False),
+                                                        (24, 64, (8, 8, 8), True), (6, 256, (64,), False)])
+def test_rope_axes_large(cuda, heads, hd, sections, adjacent):
+    """Outputs past 16 MB (streamed past the L2): rows at both ends and in the middle, and the whole against in place."""
+    from mme import ops
+    g = gen(hd)
+    rows = 20001
+    x = randn(g, rows, heads * hd)
+    pos = torch.randint(0, 5000, (len(sections), rows), generator=g, dtype=torch.int64).to(torch.int32)
+    freqs, axes = ops.rope_axes_freqs(sections, 1e4, device=cuda)
+    y = ops.rope_axes(x.to(cuda), pos.to(cuda), freqs, axes, heads, adjacent=adjacent)
+    for few in (slice(0, 40), slice(9990, 10030), slice(rows - 40, rows)):
+        check_rope(y[few], x[few], pos[:, few], freqs.cpu(), axes.cpu(), heads, hd, adjacent=adjacent)
+    z = x.to(cuda)
+    ops.rope_axes(z, pos.to(cuda), freqs, axes, heads, adjacent=adjacent, out=z)
+    assert torch.equal(z, y)
 
 
 def test_rope_axes_gradient_is_the_inverse(cuda):
