@@ -17,8 +17,8 @@
 // the operand of O^T = V^T.P^T, V^T by transposed LDS reads.
 //
 // A key outside a row's interval adds nothing to it, whatever K and V hold there: rows of another document are never
-// read, masked scores are replaced and not added to, and where a causal row comes out not finite while V holds an
-// infinity or NaN at a key that its tile has and it does not see (0 x NaN), the row is taken again from its own keys.
+// read, masked scores are replaced and not added to, and where a row comes out not finite while V holds an infinity
+// or NaN at a key that its tile has with weight 0 (0 x NaN), the row is taken again from its own keys.
 //
 // Few query rows and many keys (max_rows given): the keys of each document are split into chunks, one workgroup
 // each, which leave (maximum, sum, O) in a workspace, and a second launch joins them.
@@ -42,7 +42,7 @@ struct DocsArgs {
     float *part, *stat;  // split: O [slot][key head][flat row][hd], and (maximum, sum) [slot][key head][flat row][2]
     long ldq, ldk, ldv, ldo;
     int nslots, n, rows_q, rows_k, Hkv, group, hd, max_rows, causal, part_rows, row_blocks, sorted;
-    int per;            // a slot's flat rows (a power of two), or keys (split)
+    int per;  // a slot's flat rows, or keys (split)
     float scale_log2, cap_log2, cap_in;
 };
 
@@ -130,7 +130,7 @@ struct Tile {
     static constexpr int NKS = (HD + 15) / 16;        // k-steps of Q K^T
     static constexpr int NDB = (HD + 31) / 32;        // 32-column blocks of O^T
     // Where a row is a power of two of chunks, columns of rows would meet in the same banks: a chunk's place is XORed
-    // with bits of its row and the 1 KiB pieces (RP rows) get a gap, so that the 16 rows of a K read, and the 4 rows of
+    // with bits of its row and the 1 KiB pieces get a gap, so that the 16 rows of a K read, and the 4 rows of
     // a transposed V read (64 bytes each), take 256 bytes of banks between them. X is the XOR's unit in chunks: the
     // addresses of a lane are one register for each of its NX values (and constants), not one for each k-step.
     static constexpr bool XOR = !GEN && (HD & (HD - 1)) == 0;
@@ -197,6 +197,15 @@ __device__ __forceinline__ void row_alone(const DocsArgs& a, const Doc& D, int g
     }
 }
 
+// Whole calls measured beside a matrix product's 1 400 TF/s and a copy's 5.2 TB/s, and what bounds them:
+//   12 pages of 1 030 - 1 100 tokens, 8 heads to 1 of 256, prefix, capped: 142 - 165 us, 0.64 - 0.74 PF/s. 806
+//     workgroups over the 512 places that 256 registers leave are two rounds, the second part full; MFMA 43 % busy.
+//   14 images of 64 - 2 916 patches, 16 heads of 72: 118 - 126 us, 0.67 - 0.72 PF/s; 72 is padded to 80 and 96 columns, and
+//     the softmax's vector instructions share the issue with MFMA (50 % busy).
+//   3 texts, the longest 6 143, 32 heads to 8 of 128, causal: 296 - 322 us, 0.96 - 1.05 PF/s; MFMA 57 % busy.
+//   256 captions of 5 - 77 tokens, 12 heads of 64, biased: 15 us; a wave's chain of a copy, a product, a softmax.
+//   One query against 1 030 keys: 14 us, two launches, latency; 64 against 256 - 4 096 keys, 16 heads of 72: 92 us, 4.4 TB/s;
+//     5 against 3 001 - 65 536 keys, 8 key heads of 128: 160 us, 4.8 TB/s.
 // MODE: 1 = capped scores, 2 = biased by distance, 3 = both
 // AHEAD: the next tile's scores are formed beside this one's weights
 template <int HD, bool GEN, int NW, int MINW, bool AHEAD, bool SPLIT, int MODE>
@@ -579,7 +588,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
                 if (fr < flat && d0 < a.hd) *reinterpret_cast<uint4*>(orow + d0) = make_uint4(sx[0], sy[0], sx[1], sy[1]);
             }
     }
-    if (!a.causal) return;  // all rows saw the same keys; what the last tile had besides repeats the last of them
+    // Keys of weight 0 that the tiles had besides: those past a row's interval, and where a tile reaches past the
+    // document its last key again. 0 x infinity there may have spoilt the row.
+    const bool repeats = key_lo + (long)nkt * KT > klen;
+    if (!a.causal && !repeats) return;
 
     float nan = 0.f;
 #pragma unroll
@@ -590,16 +602,19 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     unsigned long bad = __builtin_amdgcn_ballot_w64(fr < flat && nan != 0.f);
     bad = (bad | bad >> 32) & 0xffffffffu;
     if (bad == 0) return;
-    // keys that the block's tiles had and some of this wave's rows do not see: does V hold an infinity or NaN there?
+    // does V hold an infinity or NaN at a key that some of this wave's rows do not see, or an infinity at a repeated one?
     bool found = false;
     {
         int least = hi;
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) least = min(least, __shfl_xor(least, x, 64));
         const int end = (int)min((long)klen, key_lo + (long)nkt * KT);
-        for (int j = max(least, key_lo); j < end; ++j) {
+        for (int j = min(max(least, key_lo), repeats ? klen - 1 : klen); j < end; ++j) {
             const bf16* v = a.v + (D.k0 + (long)j) * a.ldv + (long)kvh * a.hd;
-            for (int e = lane; e < a.hd; e += 64) found |= !(fabsf(bf2f(v[e])) < INFINITY);
+            for (int e = lane; e < a.hd; e += 64) {
+                const float x = fabsf(bf2f(v[e]));
+                found |= j < least ? x == INFINITY : !(x < INFINITY);
+            }
         }
     }
     if (__builtin_amdgcn_ballot_w64(found) == 0) return;
@@ -607,7 +622,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     for (int x = 0; x < 32; ++x) {
         if (!(bad >> x & 1)) continue;
         const int fx = f0 + wave * 32 + x, qx = fx / a.group, gx = kvh * a.group + fx - qx * a.group, px = qx + klen - qlen;
-        const int hx = min(klen, max(D.pre, px + 1));
+        const int hx = a.causal ? min(klen, max(D.pre, px + 1)) : klen;
         float mx, lx, acc[(HD + 63) / 64];
         row_alone<HD>(a, D, gx, kvh, px, qx, key_lo, SPLIT ? (int)min((long)hx, (long)key_lo + a.per) : hx, mx, lx, acc);
         const long at = ((long)slot * a.Hkv + kvh) * a.part_rows + fx;
@@ -625,7 +640,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
 }
 
 // Joins a document's chunks: one workgroup a (document, flat row, key head), a thread four columns of every SG-th
-// chunk, the chunks' factors 2^(m_s - max m) in LDS.
+// chunk, the chunks' factors 2^(m_s - max m) in LDS. Latency: it reads a few MB at most; 3.9 us for 8 rows of 33 chunks, 6.4
+// us for 160 rows of up to 61 (a workgroup a row keeps all of a row's loads in flight).
 __global__ __launch_bounds__(256) void join_docs_kernel(DocsArgs a) {
     __shared__ float wide[4], w[256], sums[4 * 256];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -686,7 +702,8 @@ __global__ __launch_bounds__(256) void join_docs_kernel(DocsArgs a) {
 
 struct Plan {
     bool split;
-    int NW, per, part_rows, row_blocks, nslots;
+    int NW, per, part_rows, row_blocks;
+    long nslots;
     size_t stat, ws;
 };
 
@@ -722,7 +739,7 @@ Plan make_plan(int n, int rows_q, int rows_k, int Hkv, int group, int hd, int ma
         p.stat = (size_t)nslots * Hkv * mr * hd;  // where the statistics begin, in floats
         p.ws = (p.stat + (size_t)nslots * Hkv * mr * 2) * 4;
     }
-    p.nslots = nslots * Hkv * p.row_blocks < (1L << 31) ? (int)nslots : -1;
+    p.nslots = nslots;
     return p;
 }
 
@@ -783,16 +800,19 @@ extern "C" int mme_attention_docs(const void* q, long ldq, const void* k, long l
     const int mr = max_rows < rows_q ? max_rows : rows_q;
     if (mr == 0) return MME_OK;
     const Plan p = make_plan(n, rows_q, rows_k, Hkv, Hq / Hkv, hd, mr);
-    MME_REQUIRE(p.nslots >= 0 && (long)rows_q * (Hq / Hkv) < (1L << 31) - 512 && rows_k < 0x7fff0000 && (long)n * Hkv * p.part_rows < (1L << 31),
+    // a launch has under 2^32 threads
+    MME_REQUIRE(p.nslots * Hkv * p.row_blocks * p.NW < (1L << 26) && (long)n * Hkv * p.part_rows < (1L << 24) &&
+                    (long)rows_q * (Hq / Hkv) < (1L << 31) - 512 && rows_k < 0x7fff0000,
                 "mme_attention_docs: too many rows");
     MME_REQUIRE(p.ws == 0 || (workspace && ws_bytes >= p.ws && ((uintptr_t)workspace & 15) == 0),
                 "mme_attention_docs: workspace of %zu bytes, %zu needed", ws_bytes, p.ws);
     DocsArgs a{};
     a.q = (const bf16*)q, a.k = (const bf16*)k, a.v = (const bf16*)v, a.out = (bf16*)out;
     a.qoff = q_offsets, a.koff = k_offsets, a.prefix = prefix, a.slopes = slopes, a.part = (float*)workspace, a.stat = a.part + p.stat;
-    a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldo = ldo, a.nslots = p.nslots;
+    a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldo = ldo, a.nslots = (int)p.nslots;
     a.n = n, a.rows_q = rows_q, a.rows_k = rows_k, a.Hkv = Hkv, a.group = Hq / Hkv, a.hd = hd;
-    a.sorted = !p.split && n > 1 && n <= 63 && (long)p.nslots * Hkv >= 512, a.max_rows = mr, a.causal = causal ? 1 : 0, a.per = p.per, a.part_rows = p.part_rows, a.row_blocks = p.row_blocks;
+    a.sorted = !p.split && n > 1 && n <= 63 && p.nslots * Hkv >= 512;
+    a.max_rows = mr, a.causal = causal ? 1 : 0, a.per = p.per, a.part_rows = p.part_rows, a.row_blocks = p.row_blocks;
     a.scale_log2 = scale * LOG2E;
     a.cap_log2 = softcap * LOG2E;
     a.cap_in = softcap != 0.f ? 2.0f * a.scale_log2 / softcap : 0.f;

@@ -224,7 +224,7 @@ extern "C" int mme_rope_axes(const void* x, long ldx, void* y, long ldy, int row
                         (((uintptr_t)x | (uintptr_t)y) & 3) == 0 && pairs <= 1024;
     if (!chunks) {
         const long blocks = ((long)rows * (hd - pairs) + 255) / 256;
-        MME_REQUIRE(blocks < (1L << 31), "mme_rope_axes: too many rows");
+        MME_REQUIRE(blocks < (1L << 24), "mme_rope_axes: too many rows");  // a launch has under 2^32 threads
         if (adjacent)
             hipLaunchKernelGGL(rope_axes_any_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, s, a);
         else
@@ -234,8 +234,9 @@ extern "C" int mme_rope_axes(const void* x, long ldx, void* y, long ldy, int row
     // rows a workgroup: enough for four chunks a thread, but workgroups for all CUs first, and 16 KB of LDS at most
     const long row_bytes = 2L * nheads * hd;
     long R = 16384 / row_bytes + 1;
-    if (R > (rows + 1023) / 1024) R = (rows + 1023) / 1024;
+    if (R > (rows + 1023L) / 1024) R = (rows + 1023L) / 1024;
     if (R > 2048 / pairs) R = 2048 / pairs;
+    MME_REQUIRE((rows + R - 1) / R < (1L << 24), "mme_rope_axes: too many rows");
     a.R = (int)R;
     const dim3 grid((unsigned)((rows + R - 1) / R));
     const size_t shared = (size_t)R * pairs * sizeof(float2);

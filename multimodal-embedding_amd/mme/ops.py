@@ -469,8 +469,7 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axe
     positions[axes[i], row] * freqs[i].
 
     x: bf16 [rows, >= nheads * hd] (hd defaults to x.shape[1] // nheads); positions: int32 [naxes, rows], rows of it
-    contiguous (one row expanded to all axes will do); freqs:
-    float64 [pairs]; axes: int32 [pairs] (rope_axes_freqs makes both). The pair is elements (i, i + pairs) of a head,
+    contiguous (one row expanded to all axes will do); freqs: float64 [pairs]; axes: int32 [pairs] (rope_axes_freqs makes both). The pair is elements (i, i + pairs) of a head,
     or (2i, 2i + 1) with adjacent; elements from 2 * pairs on are copied. inverse turns back: the gradient with
     respect to x is this of the gradient with respect to the result. out: None for a new tensor, x itself for in
     place, or one that does not overlap x."""
@@ -541,11 +540,11 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: t
     key head serves heads / kv_heads query heads. offsets: int32 [n + 1], where each document's query rows begin;
     key_offsets: the same for the keys (default: offsets). Query i of a document stands at key position
     i + klen - qlen. causal: it sees keys up to its own position, and with prefix (int32 [n]) also the document's
-    first prefix[d] keys. softcap (0 for none, or 1e-3 to 1e3): scores become softcap * tanh(score / softcap). slopes (fp32 [heads]): scores
-    lose slopes[h] * distance. A query that sees no key gets zeros; keys that it does not see add nothing, whatever
+    first prefix[d] keys. softcap (0 for none, or 1e-3 to 1e3): scores become softcap * tanh(score / softcap).
+    slopes (fp32 [heads]): scores lose slopes[h] * distance. A query that sees no key gets zeros; keys that it does not see add nothing, whatever
     they hold. max_rows: no document has more query rows than this; give it where rows are few and keys many (one
     query a document: max_rows=1), so that the keys are split over the device. Rows of no document, and a document's
-    rows from max_rows on, are left as they were (not set in a new out)."""
+    rows from max_rows on, are left as they were (not set in a new out). out must not overlap q, k or v."""
     key_offsets = offsets if key_offsets is None else key_offsets
     dev = q.get_device()
     if dev < 0 or not dev == k.get_device() == v.get_device() == offsets.get_device() == key_offsets.get_device() \

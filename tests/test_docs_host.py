@@ -54,6 +54,8 @@ DOCS = dict(q=16, ldq=512, k=16, ldk=128, v=16, ldv=128, out=16, ldo=512, q_off=
     (dict(v=None), "null"), (dict(k_off=None), "null"), (dict(ldq=511), "leading"), (dict(ldk=127), "leading"),
     (dict(ldo=504), "leading"), (dict(ldv=1 << 24), "2\\^24"), (dict(q=8), "misaligned"), (dict(out=24), "misaligned"),
     (dict(q_off=18), "misaligned"), (dict(rows_k=2147483647), "too many"),
+    (dict(n=20000000, Hq=16, Hkv=16, ldq=1024, ldk=1024, ldv=1024, ldo=1024), "too many"),
+    (dict(rows_q=2147483647, max_rows=2147483647), "too many"),
     (dict(n=1, rows_q=1, rows_k=60000, max_rows=1), "workspace"),
     (dict(n=1, rows_q=1, rows_k=60000, max_rows=1, ws=16, ws_bytes=100), "workspace"),
     (dict(n=1, rows_q=1, rows_k=60000, max_rows=1, ws=8, ws_bytes=1 << 40), "workspace")])
@@ -70,7 +72,9 @@ ROPE = dict(x=16, ldx=128, y=16, ldy=128, rows=4, nheads=2, hd=64, pairs=32, pos
     (dict(pairs=33), "33 pairs"), (dict(pairs=0), "0 pairs"), (dict(nheads=0), "bad shape"), (dict(rows=-1), "bad shape"),
     (dict(naxes=0), "bad shape"), (dict(ldx=127), "leading"), (dict(ldp=-1), "leading"), (dict(ldy=130), "in place"),
     (dict(x=None), "null"), (dict(freqs=None), "null"), (dict(freqs=12), "misaligned"), (dict(x=17), "misaligned"),
-    (dict(nheads=65535, hd=4096, ldx=1 << 40, ldy=1 << 40), "rows of")])
+    (dict(nheads=65535, hd=4096, ldx=1 << 40, ldy=1 << 40), "rows of"),
+    (dict(rows=2147483647, hd=4096, pairs=2048, ldx=8192, ldy=8192, ldp=2147483647), "too many"),
+    (dict(rows=2147483647, hd=2048, pairs=1024, ldx=4096, ldy=4096, ldp=2147483647), "too many")])
 def test_rope_axes_refusals(change, match):
     with pytest.raises(_lib.MMEError, match=match):
         _lib.call("mme_rope_axes", *{**ROPE, **change}.values(), None)

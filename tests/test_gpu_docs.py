@@ -375,6 +375,31 @@ def test_docs_what_masked_keys_hold_does_not_matter(cuda, hd, value):
         assert torch.isnan(got[2 + 70 + 41:2 + 160].float()).all()
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd", [(2, 1, 64), (2, 2, 72), (1, 1, 96), (2, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("split", [False, True])
+def test_docs_an_infinity_that_is_seen(cuda, heads, kv_heads, hd, causal, split):
+    """An infinity in v at a document's last key, whose tile reaches past the document: infinite in its column for
+    the rows that see it, and nowhere else."""
+    from mme import ops
+    g = gen(15)
+    klens = (1, 33, 64, 70, 2001)
+    off = cuts((1,) * 5 if split else klens).to(cuda)
+    koff = cuts(klens).to(cuda)
+    rows, keys = int(off[-1]), sum(klens)
+    q, k, v = make(g, rows, keys, heads, kv_heads, hd, cuda)
+    v[koff[1:].long() - 1, 3] = float("inf")
+    got = ops.attention_docs(q, k, v, off, heads, kv_heads, key_offsets=koff, max_rows=1 if split else None, causal=causal)
+    want, spread, _ = oracle.attention_docs(*(t.double().cpu().numpy() for t in (q, k, v)), off.cpu().numpy(), heads,
+                                            kv_heads, key_offsets=koff.cpu().numpy(), causal=causal)
+    got = got.double().cpu().numpy()
+    assert np.isinf(want).sum() >= 5 and not np.isnan(want).any()
+    assert np.array_equal(np.isposinf(got), np.isposinf(want)) and not np.isnan(got).any()
+    # check_docs' bound is at most 3 half steps of the spread, and 2 delta < 2^-9 of it with reach < 64 and hd <= 256
+    ok = np.isfinite(want)
+    assert (np.abs(got[ok] - want[ok]) <= 4 * HALF * spread[ok] + 2.0 ** -20).all()
+
+
 def test_docs_values_that_reach_far(cuda):
     """Scores of +-1e30, all alike, and a maximum that grows in every tile."""
     from mme import ops
