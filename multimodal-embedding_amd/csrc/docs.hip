@@ -155,8 +155,8 @@ struct Tile {
 };
 
 // One flat row from its own keys alone, [lo, hi) of its document, by one wave: 64 keys a step, a lane each for the
-// scores and a lane for each column of V (columns lane + 64 c in acc[c]); m in powers of two, weights not rounded. Latency: 0.14 ms for 1 100 keys of 128 (0.45
-// with one key of V at a time).
+// scores and a lane for each column of V (columns lane + 64 c in acc[c]); m in powers of two, weights not
+// rounded. Latency: 0.14 ms for 1 100 keys of 128 (0.45 with one key of V at a time).
 template <int HD>
 __device__ __forceinline__ void row_alone(const DocsArgs& a, const Doc& D, int gh, int kvh, int pq, int qi, int lo, int hi,
                                        float& m, float& l, float (&acc)[(HD + 63) / 64]) {
