@@ -743,8 +743,8 @@ Plan make_plan(int n, int rows_q, int rows_k, int Hkv, int group, int hd, int ma
     // to 4 096, 64 x 16 heads of 72: 119 and 100 us.
     const long mr = (long)max_rows * group, rb = (mr + 31) / 32, blocks = nslots * Hkv;
     const long resident = 256 * (hd <= 64 ? 4 : hd <= 80 ? 3 : 2);
-    const long parts = resident * 11 / 4 / (n * Hkv * rb);
-    if (mr <= 256 && parts >= 2 && keys * hd >= (blocks <= 128 ? 40960 : 81920)) {
+    const long parts = mr <= 256 ? resident * 11 / 4 / ((long)n * Hkv * rb) : 0;
+    if (parts >= 2 && keys * hd >= (blocks <= 128 ? 40960 : 81920)) {
         p.split = true;
         p.NW = 1;
         const long kt = hd > 128 ? 32 : 64;  // keys a tile

@@ -122,3 +122,14 @@ def test_the_oracle_against_torch():
     y, _ = oracle.rope_axes(x, np.array([[1, 2, 3], [5, 7, 9]]), [1.0, 0.5], [0, 1], 2, 4, adjacent=True)
     z = (x[:, 0::2] + 1j * x[:, 1::2]) * np.exp(1j * np.array([[1.0, 2.5], [2.0, 3.5], [3.0, 4.5]]))[:, [0, 1, 0, 1]]
     assert np.allclose(y[:, 0::2], z.real, atol=1e-14) and np.allclose(y[:, 1::2], z.imag, atol=1e-14)
+
+
+@pytest.mark.parametrize("n,rows,Hq,Hkv", [(1 << 30, 1, 4, 4), (1 << 28, 1 << 28, 16, 16), (1 << 30, 1 << 30, 8, 4),
+                                           (1 << 30, 1, 8, 8), (2147483647, 2147483647, 65535, 65535)])
+def test_products_of_documents_and_key_heads_past_32_bits(n, rows, Hq, Hkv):
+    """A product that is a multiple of 2^32 was a division by zero: the sizes are answered, the call is refused."""
+    assert ws(n, rows, rows, Hq, Hkv, 64, 1) == 0
+    wide = dict(ldq=Hq * 64, ldk=Hkv * 64, ldv=Hkv * 64, ldo=Hq * 64)
+    with pytest.raises(_lib.MMEError, match="too many"):
+        _lib.call("mme_attention_docs", *{**DOCS, **wide, "n": n, "rows_q": rows, "rows_k": rows, "Hq": Hq, "Hkv": Hkv,
+                                          "max_rows": 1}.values(), None)
