@@ -468,8 +468,9 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axe
     """Rotary positions with several axes (mme_rope_axes): pair i of heads [0, nheads) of each row turns by
     positions[axes[i], row] * freqs[i].
 
-    x: bf16 [rows, >= nheads * hd] (hd defaults to x.shape[1] // nheads); positions: int32 [naxes, rows], rows of it
-    contiguous (one row expanded to all axes will do); freqs: float64 [pairs]; axes: int32 [pairs] (rope_axes_freqs makes both). The pair is elements (i, i + pairs) of a head,
+    x: bf16 [rows, >= nheads * hd]; hd may be left out where the heads are the whole row; positions: int32
+    [naxes, rows], rows of it contiguous (one row expanded to all axes will do); freqs: float64 [pairs]; axes: int32
+    [pairs] (rope_axes_freqs makes both). The pair is elements (i, i + pairs) of a head,
     or (2i, 2i + 1) with adjacent; elements from 2 * pairs on are copied. inverse turns back: the gradient with
     respect to x is this of the gradient with respect to the result. out: None for a new tensor, x itself for in
     place, or one that does not overlap x."""
@@ -482,7 +483,10 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axe
             return rope_axes(x, positions, freqs, axes, nheads, hd=hd, adjacent=adjacent, inverse=inverse, out=out)
     ldx = _rowmajor(x, "x")
     (rows, width), pairs = x.shape, freqs.numel()
-    hd = width // max(nheads, 1) if hd is None else hd
+    if hd is None:
+        if nheads < 1 or width % nheads:
+            raise ValueError(f"rope_axes: rows of {width} are not {nheads} heads: hd says how wide a head is")
+        hd = width // nheads
     if x.dtype is not BF16:
         raise ValueError("rope_axes: x must be bf16")
     if nheads < 1 or pairs < 1 or 2 * pairs > hd or nheads * hd > width:

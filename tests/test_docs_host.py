@@ -133,3 +133,35 @@ def test_products_of_documents_and_key_heads_past_32_bits(n, rows, Hq, Hkv):
     with pytest.raises(_lib.MMEError, match="too many"):
         _lib.call("mme_attention_docs", *{**DOCS, **wide, "n": n, "rows_q": rows, "rows_k": rows, "Hq": Hq, "Hkv": Hkv,
                                           "max_rows": 1}.values(), None)
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that says it lies on device 0: the wrappers' own checks run without a GPU."""
+
+    def get_device(self):
+        return 0
+
+
+@pytest.fixture
+def no_launch(monkeypatch):
+    calls = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(ops, "call", lambda *args: calls.append(args))
+    return calls
+
+
+def here(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(OnDevice)
+
+
+def test_rope_axes_heads_that_do_not_divide_a_row(no_launch):
+    """9 heads of 72 and 16 more columns are not 9 heads of 73; with hd given they are what they are."""
+    f, a = (t.as_subclass(OnDevice) for t in ops.rope_axes_freqs((18, 18), 1e4, device="cpu"))
+    x, pos = here(4, 9 * 72 + 16), here(2, 4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="9 heads"):
+        ops.rope_axes(x, pos, f, a, 9)
+    assert not no_launch
+    assert ops.rope_axes(x, pos, f, a, 9, hd=72).shape == (4, 648)
+    assert ops.rope_axes(x[:, :648], pos, f, a, 9).shape == (4, 648)
+    assert [c[7] for c in no_launch] == [72, 72]
