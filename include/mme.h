@@ -395,7 +395,7 @@ int mme_attention_mqa(const void* qkv, int ld_qkv, void* out, int ld_out, int B,
  * reduced in 64 bits):  y_a = x_a cos - x_b sin, y_b = x_b cos + x_a sin, fp32, one rounding to bf16;
  * (a, b) = (i, i + pairs), or (2i, 2i + 1) with `adjacent`. `inverse` turns back (the rotation's gradient).
  * Elements 2*pairs .. hd of a head are copied. y may be x (ldy == ldx; those elements then stay untouched) or
- * must not overlap it. axes[i] outside [0, naxes) is clamped; ld_pos may be 0 (one row of positions for all). Any
+ * must not share an element with it (refused). axes[i] outside [0, naxes) is clamped; ld_pos may be 0 (one row of positions for all). Any
  * pairs, hd, leading dims and 2-byte alignment; fast where hd % 8 == 0, pairs % 4 == 0, the leading dims are even and pointers 4-byte aligned. */
 int mme_rope_axes(const void* x, long ldx, void* y, long ldy, int rows, int nheads, int hd, int pairs,
                   const int32_t* positions, long ld_pos, int naxes, const double* freqs, const int32_t* axes,
@@ -412,7 +412,8 @@ int mme_rope_axes(const void* x, long ldx, void* y, long ldy, int rows, int nhea
  * device and joined). q: bf16 [rows_q, ldq], head h at column h*hd; k, v: bf16 [rows_k, ld], key head h / (Hq/Hkv);
  * out: bf16 [rows_q, ldo]. hd: multiples of 8 up to 128, of 16 up to 256. 16-byte aligned pointers, leading dims
  * % 8 == 0, those of k and v under 2^24. fp32 scores, softmax and sums; the weights are rounded to bf16 for the matrix
- * instruction. out must not overlap q, k or v.
+ * instruction. out must not share an element with q, k or v
+ * (refused; columns of one buffer are no overlap).
  * workspace >= mme_attention_docs_workspace_bytes(...); 0 (it may be null), unless max_rows * Hq / Hkv <= 256 and
  * rows_k * hd >= 40960 * n. */
 size_t mme_attention_docs_workspace_bytes(int n, int rows_q, int rows_k, int Hq, int Hkv, int hd, int max_rows);

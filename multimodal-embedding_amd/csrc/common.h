@@ -27,6 +27,8 @@ typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
 // ---------------------------------------------------------------------------
 int mme_set_error(int code, const char* fmt, ...);
 int mme_check_launch(const char* what);
+// do two blocks of rows of 2-byte elements (leading dim, rows, width) share an element?
+bool mme_rows_overlap(const void* a, long lda, long ra, long wa, const void* b, long ldb, long rb, long wb);
 
 #define MME_REQUIRE(cond, ...)                                  \
     do {                                                        \

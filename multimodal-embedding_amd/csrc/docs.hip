@@ -821,6 +821,11 @@ extern "C" int mme_attention_docs(const void* q, long ldq, const void* k, long l
                 "mme_attention_docs: too many rows");
     MME_REQUIRE(p.ws == 0 || (workspace && ws_bytes >= p.ws && ((uintptr_t)workspace & 15) == 0),
                 "mme_attention_docs: workspace of %zu bytes, %zu needed", ws_bytes, p.ws);
+    const long wq = (long)Hq * hd, wk = (long)Hkv * hd;
+    MME_REQUIRE(!mme_rows_overlap(out, ldo, rows_q, wq, q, ldq, rows_q, wq) &&
+                    !mme_rows_overlap(out, ldo, rows_q, wq, k, ldk, rows_k, wk) &&
+                    !mme_rows_overlap(out, ldo, rows_q, wq, v, ldv, rows_k, wk),
+                "mme_attention_docs: out overlaps q, k or v");
     DocsArgs a{};
     a.q = (const bf16*)q, a.k = (const bf16*)k, a.v = (const bf16*)v, a.out = (bf16*)out;
     a.qoff = q_offsets, a.koff = k_offsets, a.prefix = prefix, a.slopes = slopes, a.part = (float*)workspace, a.stat = a.part + p.stat;

@@ -218,6 +218,8 @@ extern "C" int mme_rope_axes(const void* x, long ldx, void* y, long ldy, int row
     MME_REQUIRE(((uintptr_t)x & 1) == 0 && ((uintptr_t)y & 1) == 0 && ((uintptr_t)positions & 3) == 0 &&
                     ((uintptr_t)axes & 3) == 0 && ((uintptr_t)freqs & 7) == 0,
                 "mme_rope_axes: misaligned pointer");
+    MME_REQUIRE(x == y || !mme_rows_overlap(x, ldx, rows, (long)nheads * hd, y, ldy, rows, (long)nheads * hd),
+                "mme_rope_axes: x and y overlap");
     RopeArgs a{(const bf16*)x, (bf16*)y, positions, freqs, axes, ldx, ldy, ld_pos, rows, nheads, hd, pairs, naxes, 0,
                inverse ? -1.0f : 1.0f};
     hipStream_t s = as_stream(stream);

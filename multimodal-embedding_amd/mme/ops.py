@@ -473,7 +473,7 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axe
     [pairs] (rope_axes_freqs makes both). The pair is elements (i, i + pairs) of a head,
     or (2i, 2i + 1) with adjacent; elements from 2 * pairs on are copied. inverse turns back: the gradient with
     respect to x is this of the gradient with respect to the result. out: None for a new tensor, x itself for in
-    place, or one that does not overlap x."""
+    place, or one that shares no element with x."""
     dev = x.get_device()
     if dev < 0 or not dev == positions.get_device() == freqs.get_device() == axes.get_device() \
             or (out is not None and out.get_device() != dev):
@@ -548,7 +548,8 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: t
     slopes (fp32 [heads]): scores lose slopes[h] * distance. A query that sees no key gets zeros; keys that it does not see add nothing, whatever
     they hold. max_rows: no document has more query rows than this; give it where rows are few and keys many (one
     query a document: max_rows=1), so that the keys are split over the device. Rows of no document, and a document's
-    rows from max_rows on, are left as they were (not set in a new out). out must not overlap q, k or v."""
+    rows from max_rows on, are left as they were (not set in a new out). out must not share an element with q, k
+    or v (other columns of their buffer will do)."""
     key_offsets = offsets if key_offsets is None else key_offsets
     dev = q.get_device()
     if dev < 0 or not dev == k.get_device() == v.get_device() == offsets.get_device() == key_offsets.get_device() \

@@ -165,3 +165,25 @@ def test_rope_axes_heads_that_do_not_divide_a_row(no_launch):
     assert ops.rope_axes(x, pos, f, a, 9, hd=72).shape == (4, 648)
     assert ops.rope_axes(x[:, :648], pos, f, a, 9).shape == (4, 648)
     assert [c[7] for c in no_launch] == [72, 72]
+
+
+AT = 1 << 20
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=AT), dict(k=AT), dict(v=AT), dict(q=AT + 7 * 1024 + 1008), dict(v=AT - 7 * 256 - 112, ldv=128),
+    dict(q=AT + 1008, ldo=1024, ldq=1024), dict(k=AT + 992, ldo=1024, ldk=1024), dict(k=AT - 240, ldo=1024, ldk=1024),
+    dict(v=AT + 4096 - 16, ldo=1024, ldv=2048), dict(q=AT + 6 * 2048 + 1008, ldo=1024, ldq=4096)])
+def test_attention_docs_refuses_an_out_over_its_inputs(change):
+    """out is 8 rows of 1 024 bytes, k and v 8 of 256; what a change moves meets it by 16 bytes or more."""
+    apart = dict(q=1 << 30, k=2 << 30, v=3 << 30, out=AT)
+    with pytest.raises(_lib.MMEError, match="overlap"):
+        _lib.call("mme_attention_docs", *{**DOCS, **apart, **change}.values(), None)
+
+
+@pytest.mark.parametrize("change", [dict(y=AT + 2), dict(y=AT - 254), dict(y=AT + 256 * 3 + 254), dict(y=AT + 254, ldx=256, ldy=256),
+                                    dict(y=AT + 2 * 256 + 16, ldx=256, ldy=384)])
+def test_rope_axes_refuses_rows_that_overlap(change):
+    """4 rows of 256 bytes, turned into rows that share some but not all of their places with them."""
+    with pytest.raises(_lib.MMEError, match="overlap"):
+        _lib.call("mme_rope_axes", *{**ROPE, "x": AT, **change}.values(), None)

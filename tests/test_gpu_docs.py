@@ -571,3 +571,31 @@ def test_a_decoder_step_over_packed_pages(cuda):
     one = cuts([1] * len(pages)).to(cuda)
     alone = ops.attention_docs(q[last].contiguous(), k, v, one, H, 1, key_offsets=off, max_rows=1, **kw)
     check_docs(alone, q[last], k, v, one, H, 1, key_offsets=off, **kw)
+
+
+def test_out_beside_its_inputs_and_over_them(cuda):
+    """Columns of one buffer are no overlap, at one leading dim or two; shared elements are refused before any launch."""
+    from mme import _lib, ops
+    g = gen(31)
+    lens = (70, 33, 5)
+    off = cuts(lens).to(cuda)
+    buf = torch.zeros(108, 1024, dtype=BF16, device=cuda)
+    buf[:, :512] = randn(g, 108, 512).to(cuda)
+    q, k, v = buf[:, :256], buf[:, 256:384], buf[:, 384:512]
+    keep = buf[:, :512].clone()
+    want = ops.attention_docs(*(t.contiguous() for t in (q, k, v)), off, 4, 2, causal=True)
+    assert torch.equal(ops.attention_docs(q, k, v, off, 4, 2, causal=True, out=buf[:, 512:768]), want)
+    wide = torch.zeros(216, 512, dtype=BF16, device=cuda)   # rows of out at every other row of k
+    kk = wide[:, 256:384].copy_(k.repeat_interleave(2, 0))
+    two = ops.attention_docs(q, kk, kk, off, 4, 2, key_offsets=off * 2, out=wide.view(108, 1024)[:, :256])
+    assert torch.equal(two, ops.attention_docs(q, kk.contiguous(), kk.contiguous(), off, 4, 2, key_offsets=off * 2))
+    f, a = ops.rope_axes_freqs((32,), 1e4, device=cuda)
+    pos = torch.arange(108, dtype=torch.int32, device=cuda)[None]
+    assert torch.equal(ops.rope_axes(q, pos, f, a, 4, out=buf[:, 768:]), ops.rope_axes(q.contiguous(), pos, f, a, 4))
+    assert torch.equal(buf[:, :512], keep)
+    for bad in (lambda: ops.attention_docs(q, k, v, off, 4, 2, out=q), lambda: ops.attention_docs(q, k, v, off, 4, 2, out=buf[:, 376:632]),
+                lambda: ops.rope_axes(q, pos, f, a, 4, out=buf[:, 64:320]),
+                lambda: ops.rope_axes(buf[:100, :256], pos[:, :100], f, a, 4, out=buf[1:101, :256])):
+        with pytest.raises(_lib.MMEError, match="overlap"):
+            bad()
+    assert torch.equal(buf[:, :512], keep)
