@@ -404,7 +404,8 @@ int mme_rope_axes(const void* x, long ldx, void* y, long ldy, int rows, int nhea
 /* Attention over n packed documents. Document d has the query rows [q_offsets[d], q_offsets[d+1]) and the key rows
  * [k_offsets[d], k_offsets[d+1]); the offsets (int32[n+1], not decreasing; clamped to the rows there are) may be the
  * same array. Query i of a document stands at key position p = i + klen - qlen. It sees key j of its own document
- * where  !causal,  or j <= p,  or j < prefix[d] (int32[n], nullable, with causal only). Its score is
+ * where  !causal,  or j <= p,  or j < prefix[d] (int32[n], nullable, with causal only). Its score is (scale > 0; its
+ * products with log2(e), and with 2 log2(e) / softcap, must be finite)
  *   x = scale q.k;  softcap (0, or 1e-3 .. 1e3): x = softcap tanh(x / softcap);  slopes (fp32[Hq], nullable): x -= slopes[h] |p - j|
  * and out = softmax(x) v over the keys it sees, 0 where it sees none. A key that a query does not see adds nothing
  * to it, whatever k and v hold there. Rows of no document are left as they were, and so are a document's rows from

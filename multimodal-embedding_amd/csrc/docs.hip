@@ -802,6 +802,8 @@ extern "C" int mme_attention_docs(const void* q, long ldq, const void* k, long l
     if (int rc = check_docs(n, rows_q, rows_k, Hq, Hkv, hd, max_rows)) return rc;
     MME_REQUIRE(scale > 0.f && scale < INFINITY, "mme_attention_docs: scale must be positive and finite");
     MME_REQUIRE(softcap == 0.f || (softcap >= 1e-3f && softcap <= 1e3f), "mme_attention_docs: softcap must be 0 (none) or from 1e-3 to 1e3");
+    const float scale_log2 = scale * LOG2E, cap_in = softcap != 0.f ? 2.0f * scale_log2 / softcap : 0.f;
+    MME_REQUIRE(scale_log2 < INFINITY && cap_in < INFINITY, "mme_attention_docs: scale too large (%g, softcap %g)", scale, softcap);
     MME_REQUIRE(causal || !prefix, "mme_attention_docs: a prefix goes with the causal mask");
     if (n == 0 || rows_q == 0) return MME_OK;
     MME_REQUIRE(q && out && q_offsets && k_offsets && (rows_k == 0 || (k && v)), "mme_attention_docs: null pointer");
@@ -833,9 +835,9 @@ extern "C" int mme_attention_docs(const void* q, long ldq, const void* k, long l
     a.n = n, a.rows_q = rows_q, a.rows_k = rows_k, a.Hkv = Hkv, a.group = Hq / Hkv, a.hd = hd;
     a.sorted = !p.split && n > 1 && n <= 63 && p.nslots * Hkv >= 512;
     a.max_rows = mr, a.causal = causal ? 1 : 0, a.per = p.per, a.part_rows = p.part_rows, a.row_blocks = p.row_blocks;
-    a.scale_log2 = scale * LOG2E;
+    a.scale_log2 = scale_log2;
     a.cap_log2 = softcap * LOG2E;
-    a.cap_in = softcap != 0.f ? 2.0f * a.scale_log2 / softcap : 0.f;
+    a.cap_in = cap_in;
     hipStream_t s = as_stream(stream);
     switch (hd) {
         case 64: launch_width<64, false, 3, false>(a, p, s); break;

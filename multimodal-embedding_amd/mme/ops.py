@@ -545,8 +545,8 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: t
     key_offsets: the same for the keys (default: offsets). Query i of a document stands at key position
     i + klen - qlen. causal: it sees keys up to its own position, and with prefix (int32 [n]) also the document's
     first prefix[d] keys. softcap (0 for none, or 1e-3 to 1e3): scores become softcap * tanh(score / softcap).
-    slopes (fp32 [heads]): scores lose slopes[h] * distance. A query that sees no key gets zeros; keys that it does not see add nothing, whatever
-    they hold. max_rows: no document has more query rows than this; give it where rows are few and keys many (one
+    slopes (fp32 [heads]): scores lose slopes[h] * distance. scale: positive (default: hd ** -0.5). A query that sees no
+    key gets zeros; keys that it does not see add nothing, whatever they hold. max_rows: no document has more query rows than this; give it where rows are few and keys many (one
     query a document: max_rows=1), so that the keys are split over the device. Rows of no document, and a document's
     rows from max_rows on, are left as they were (not set in a new out). out must not share an element with q, k
     or v (other columns of their buffer will do)."""

@@ -187,3 +187,10 @@ def test_rope_axes_refuses_rows_that_overlap(change):
     """4 rows of 256 bytes, turned into rows that share some but not all of their places with them."""
     with pytest.raises(_lib.MMEError, match="overlap"):
         _lib.call("mme_rope_axes", *{**ROPE, "x": AT, **change}.values(), None)
+
+
+@pytest.mark.parametrize("change", [dict(scale=3e38), dict(scale=1e36, softcap=1e-3), dict(scale=1.2e38, softcap=1.0)])
+def test_scales_whose_products_leave_32_bits_are_refused(change):
+    """scale log2(e), or 2 log2(e) scale / softcap, infinite in fp32: a score of 0 would come out as 0 x infinity."""
+    with pytest.raises(_lib.MMEError, match="scale"):
+        _lib.call("mme_attention_docs", *{**DOCS, "out": 1 << 20, "q": 1 << 21, "k": 1 << 22, "v": 1 << 23, **change}.values(), None)
