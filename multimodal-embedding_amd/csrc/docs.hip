@@ -616,7 +616,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-            if (32 * db + 8 * (e >> 2) < HD) nan = __builtin_fmaf(o[db][e], 0.f, nan);
+            if (32 * db + 8 * (e >> 2) < (GEN ? a.hd : HD)) nan = __builtin_fmaf(o[db][e], 0.f, nan);
     unsigned long bad = __builtin_amdgcn_ballot_w64(fr < flat && nan != 0.f);
     bad = (bad | bad >> 32) & 0xffffffffu;
     if (bad == 0) return;
