@@ -771,12 +771,11 @@ void launch_docs(const DocsArgs& a, hipStream_t s) {
 
 template <int HD, bool GEN, int MINW, bool AHEAD>
 void launch_width(const DocsArgs& a, const Plan& p, hipStream_t s) {
-    if (p.split)
-        launch_docs<HD, GEN, 1, 1, false, true>(a, s);
-    else if (HD <= 128 && p.NW == 1)
-        launch_docs<HD <= 128 ? HD : 64, GEN, 1, HD <= 80 ? 2 : 1, false, false>(a, s);
-    else
-        launch_docs<HD, GEN, 4, MINW, AHEAD, false>(a, s);
+    if (p.split) return launch_docs<HD, GEN, 1, 1, false, true>(a, s);
+    if constexpr (HD <= 128) {
+        if (p.NW == 1) return launch_docs<HD, GEN, 1, HD <= 80 ? 2 : 1, false, false>(a, s);
+    }
+    launch_docs<HD, GEN, 4, MINW, AHEAD, false>(a, s);
 }
 
 int check_docs(int n, int rows_q, int rows_k, int Hq, int Hkv, int hd, int max_rows) {

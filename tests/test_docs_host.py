@@ -1,5 +1,7 @@
 """Packed documents on the host: workspace sizes, refusals of the C entries (checked before any launch), frequencies
 and the oracle itself (no GPU)."""
+import re
+
 import numpy as np
 import pytest
 import torch
@@ -194,3 +196,12 @@ def test_scales_whose_products_leave_32_bits_are_refused(change):
     """scale log2(e), or 2 log2(e) scale / softcap, infinite in fp32: a score of 0 would come out as 0 x infinity."""
     with pytest.raises(_lib.MMEError, match="scale"):
         _lib.call("mme_attention_docs", *{**DOCS, "out": 1 << 20, "q": 1 << 21, "k": 1 << 22, "v": 1 << 23, **change}.values(), None)
+
+
+def test_no_kernel_that_nothing_launches():
+    """One-wave workgroups with whole keys are for head dims to 128: the wide head dims make no kernel of that form."""
+    with open(_lib.LIB_PATH, "rb") as f:
+        names = set(re.findall(rb"attn_docs_kernelILi(\d+)ELb([01])ELi(\d+)ELi(\d+)ELb([01])ELb([01])ELi([0-3])E", f.read()))
+    assert len({n[:2] for n in names}) == 8      # five head dims of their own, three general widths
+    # a head dim has the split form and the one for four waves, up to 128 the one for one wave too; four scores each
+    assert len(names) == 4 * (6 * 3 + 2 * 2)
