@@ -462,6 +462,12 @@ def _elsewhere(name: str, t: torch.Tensor, *ts: Optional[torch.Tensor]) -> None:
             raise ValueError(f"{name}: tensors on two devices: {t.device} and {u.device}")
 
 
+def _ld(t: torch.Tensor, name: str, width: int) -> int:
+    """_rowmajor, but a lone row lies where it begins, whatever its stride says."""
+    ld = _rowmajor(t, name)
+    return ld if t.shape[0] > 1 else width
+
+
 def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axes: torch.Tensor, nheads: int, *,
               hd: Optional[int] = None, adjacent: bool = False, inverse: bool = False,
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -481,7 +487,7 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axe
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return rope_axes(x, positions, freqs, axes, nheads, hd=hd, adjacent=adjacent, inverse=inverse, out=out)
-    ldx = _rowmajor(x, "x")
+    _rowmajor(x, "x")
     (rows, width), pairs = x.shape, freqs.numel()
     if hd is None:
         if nheads < 1 or width % nheads:
@@ -499,13 +505,14 @@ def rope_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, axe
     if freqs.dtype is not torch.float64 or axes.dtype is not torch.int32 or axes.shape != freqs.shape \
             or freqs.dim() != 1 or not (freqs.is_contiguous() and axes.is_contiguous()):
         raise ValueError("rope_axes: freqs must be contiguous float64 [pairs] and axes int32 [pairs]")
+    ldx = _ld(x, "x", nheads * hd)
     if out is None:
         out = torch.empty(rows, nheads * hd, dtype=BF16, device=x.device)
         ldo = nheads * hd
     elif out.dtype is not BF16 or out.dim() != 2 or out.shape[0] != rows or out.shape[1] < nheads * hd:
         raise ValueError(f"rope_axes: out must be bf16 [{rows}, >= {nheads * hd}]")
     else:
-        ldo = _rowmajor(out, "out")
+        ldo = _ld(out, "out", nheads * hd)
     ev = KernelTimer.begin()
     call("mme_rope_axes", x.data_ptr(), ldx, out.data_ptr(), ldo, rows, nheads, hd, pairs, positions.data_ptr(),
          ldp, naxes, freqs.data_ptr(), axes.data_ptr(), adjacent, inverse, _raw_stream(dev))
@@ -592,14 +599,16 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: t
     elif out.dtype is not BF16 or out.dim() != 2 or out.shape[0] != rows or out.shape[1] < width:
         raise ValueError(f"attention_docs: out must be bf16 [{rows}, >= {width}]")
     else:
-        ldo = _rowmajor(out, "out")
+        ldo = _ld(out, "out", width)
+    # a lone row lies where it begins, whatever its stride says
+    ldq, (ldk, ldv) = sq[0] if rows > 1 else width, (sk[0], sv[0]) if keys > 1 else (kwidth, kwidth)
     ws, wsb = None, 0
     if max_rows * heads <= 256 * kv_heads and keys * hd >= 40960 * n:  # none is needed otherwise (mme.h)
         wsb = query("mme_attention_docs_workspace_bytes", n, rows, keys, heads, kv_heads, hd, max_rows)
         # a workspace of the call's own: calls on two streams, or in two captured graphs, share none
         ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
     ev = KernelTimer.begin()
-    call("mme_attention_docs", q.data_ptr(), sq[0], k.data_ptr(), sk[0], v.data_ptr(), sv[0], out.data_ptr(), ldo,
+    call("mme_attention_docs", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo,
          offsets.data_ptr(), key_offsets.data_ptr(), n, rows, keys, heads, kv_heads, hd, max_rows, bool(causal),
          _ptr(prefix), softcap, _ptr(slopes), hd ** -0.5 if scale is None else scale, _ptr(ws), wsb, _raw_stream(dev))
     if ev is not None:

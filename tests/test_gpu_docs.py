@@ -631,3 +631,27 @@ def test_docs_time_does_not_hang_on_what_lds_held(cuda, hd, full):
     zeros, nans = (least_time(call, before) for before in runs)
     assert nans <= 1.4 * zeros, (zeros, nans)
     assert torch.equal(call(), want)
+
+
+def test_one_row_whatever_its_stride(cuda):
+    """A single row lies where it begins: a stride that leads nowhere (expanded, or odd) does not matter."""
+    from mme import ops
+    g = gen(37)
+    one = cuts((1,)).to(cuda)
+    f, a = ops.rope_axes_freqs((32,), 1e4, device=cuda)
+    pos = torch.full((1, 1), 9, dtype=torch.int32, device=cuda)
+    row = randn(g, 512).to(cuda)
+    for x in (row[:256].expand(1, 256), torch.as_strided(row, (1, 256), (771, 1), 8), torch.as_strided(row, (1, 256), (3, 1), 256)):
+        flat = x.reshape(256).clone()[None]
+        k = flat[:, :128]
+        want = ops.attention_docs(flat, k, k, one, 4, 2)
+        kk = x[:, :128]
+        assert torch.equal(ops.attention_docs(x, kk, kk, one, 4, 2), want)
+        assert torch.equal(want, torch.cat([k[:, :64], k[:, :64], k[:, 64:], k[:, 64:]], 1))
+        out = torch.as_strided(torch.zeros(800, dtype=BF16, device=cuda), (1, 256), (13, 1), 16)
+        assert torch.equal(ops.attention_docs(x, kk, kk, one, 4, 2, out=out), want)
+        turned = ops.rope_axes(flat, pos, f, a, 4)
+        assert torch.equal(ops.rope_axes(x, pos, f, a, 4), turned)
+        assert torch.equal(ops.rope_axes(x, pos, f, a, 4, out=out), turned)
+        y = flat.clone()
+        assert torch.equal(ops.rope_axes(y, pos, f, a, 2, hd=64, out=y[:, :128]), turned[:, :128])
