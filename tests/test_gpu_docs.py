@@ -655,3 +655,127 @@ def test_one_row_whatever_its_stride(cuda):
         assert torch.equal(ops.rope_axes(x, pos, f, a, 4, out=out), turned)
         y = flat.clone()
         assert torch.equal(ops.rope_axes(y, pos, f, a, 2, hd=64, out=y[:, :128]), turned[:, :128])
+
+
+# ------------------------------------------------------------------ forms that the tests above do not reach
+def check_whole(got, q, k, v, off, koff, heads, kv_heads, adds, causal=False, prefix=None, softcap=0.0, slopes=None):
+    """Whole outputs against float64 on the device, a document and a head at a time. The bound is check_docs', with
+    `adds` fp32 additions in a row's sums of weights and of products."""
+    hd = q.shape[1] // heads
+    got, off, koff = got.double(), off.tolist(), koff.tolist()
+    for d in range(len(off) - 1):
+        m, n = off[d + 1] - off[d], koff[d + 1] - koff[d]
+        p = torch.arange(m, device=q.device)[:, None] + n - m
+        at = torch.arange(n, device=q.device)[None, :]
+        seen = at >= 0 if not causal else at <= p if prefix is None else (at <= p) | (at < prefix[d])
+        for h in range(heads if m else 0):
+            j = h * kv_heads // heads
+            qq = q[off[d]:off[d + 1], h * hd:(h + 1) * hd].double().contiguous()
+            kk, vv = (t[koff[d]:koff[d + 1], j * hd:(j + 1) * hd].double().contiguous() for t in (k, v))
+            s = qq @ kk.t().contiguous() * hd ** -0.5
+            big = qq.abs() @ kk.abs().t().contiguous() * hd ** -0.5
+            if softcap:
+                s = softcap * torch.tanh(s / softcap)
+            if slopes is not None:
+                bias = slopes[h].double() * (p - at).abs()
+                s, big = s - bias, big + bias
+            s = s.masked_fill(~seen, -float("inf"))
+            w = torch.softmax(s, -1) if n else s
+            w = w.masked_fill(~seen, 0.0)   # a row that sees nothing
+            want, spread = w @ vv, w @ vv.abs()
+            reach = big.masked_fill(~seen, 0.0).amax(1, keepdim=True) if n else 0.0
+            delta = (hd + 4) * 2.0 ** -24 * reach + 3 * softcap * 2.0 ** -23 + 2.0 ** -20
+            tol = HALF * (spread + 2 * want.abs()) + 2 * (spread + want.abs()) * delta + 2 * adds * 2.0 ** -24 * spread
+            bad = ~((got[off[d]:off[d + 1], h * hd:(h + 1) * hd] - want).abs() <= tol)
+            assert not bad.any(), (d, h, bad.nonzero()[:5])
+
+
+def scores(mask, heads, klens, cuda):
+    kw = dict(causal=mask != "all")
+    if mask != "all" and "prefix" in mask:
+        kw["prefix"] = torch.tensor([(n // 2, 0, n + 3)[i % 3] for i, n in enumerate(klens)], dtype=torch.int32, device=cuda)
+    if "cap" in mask:
+        kw["softcap"] = 30.0
+    if "bias" in mask:
+        kw["slopes"] = (2.0 ** -torch.arange(2, heads + 2).float()).to(cuda)
+    return kw
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", [(4, 4, 8), (4, 4, 40), (6, 6, 64), (4, 4, 72), (8, 4, 72), (10, 5, 80), (5, 5, 96),
+                                               (6, 6, 120), (8, 4, 128), (8, 8, 128)])
+@pytest.mark.parametrize("mask", ["all", "causal", "prefix", "cap bias", "cap bias prefix"])
+def test_docs_many_short_documents(cuda, heads, kv_heads, hd, mask):
+    """96 documents of 1 to 128 rows: one wave a workgroup, tiles of 32 keys, up to four of them a document."""
+    from mme import ops
+    r = np.random.RandomState(hd)
+    lens = np.concatenate([r.randint(1, 100, 88), [1, 31, 32, 33, 64, 96, 97, 128]]).tolist()
+    rows = sum(lens)
+    assert rows * (heads // kv_heads) <= 128 * 96 and (rows * (heads // kv_heads) // 32 + 96) * kv_heads >= 512
+    g = gen(hd * 5 + heads)
+    q, k, v = make(g, rows, rows, heads, kv_heads, hd, cuda)
+    off = cuts(lens).to(cuda)
+    kw = scores(mask, heads, lens, cuda)
+    out = torch.full((rows, heads * hd), float("nan"), dtype=BF16, device=cuda)
+    check_whole(ops.attention_docs(q, k, v, off, heads, kv_heads, out=out, **kw), q, k, v, off, off, heads, kv_heads, 128, **kw)
+    # a few rows a document against up to 250 keys, some documents without keys
+    klens = r.randint(0, 250, 96).tolist()
+    qlens = r.randint(0, 40, 96).tolist()
+    q, k, v = make(g, sum(qlens), sum(klens), heads, kv_heads, hd, cuda)
+    off, koff = cuts(qlens).to(cuda), cuts(klens).to(cuda)
+    kw = scores(mask, heads, klens, cuda)
+    out = torch.full((sum(qlens), heads * hd), float("nan"), dtype=BF16, device=cuda)
+    got = ops.attention_docs(q, k, v, off, heads, kv_heads, key_offsets=koff, out=out, **kw)
+    check_whole(got, q, k, v, off, koff, heads, kv_heads, 250, **kw)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,klens", [(8, 1, 256, (20000,)), (1, 1, 64, (65536,)), (1, 1, 64, (16385, 7, 32768)),
+                                                     (4, 1, 72, (50001,)), (2, 1, 40, (40000,))])
+@pytest.mark.parametrize("mask", ["all", "cap bias prefix"])
+@pytest.mark.parametrize("far", [False, True])
+def test_docs_join_of_many_chunks(cuda, heads, kv_heads, hd, klens, mask, far):
+    """A document in hundreds of chunks (32 keys at head dim 256, 64 below: 512 to 1 024), which the join takes 256 at a
+    time; with far, a key well past the first 256 chunks has nearly all the weight."""
+    from mme import ops
+    g = gen(hd + sum(klens))
+    n = len(klens)
+    q, k, v = make(g, 3 * n, sum(klens), heads, kv_heads, hd, cuda)
+    off, koff = cuts([3] * n).to(cuda), cuts(klens).to(cuda)
+    if far:
+        for d in range(n):
+            k[int(koff[d]) + klens[d] * 4 // 5, :hd] = q[3 * d + 1, :hd] * 4
+    kw = scores(mask, heads, klens, cuda)
+    if "slopes" in kw:
+        kw["slopes"] = kw["slopes"] / 1000
+    got = ops.attention_docs(q, k, v, off, heads, kv_heads, key_offsets=koff, max_rows=3, **kw)
+    check_whole(got, q, k, v, off, koff, heads, kv_heads, 64 + 1024, **kw)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", [(4, 2, 64), (2, 2, 72), (3, 3, 96), (4, 1, 128), (4, 1, 256), (2, 1, 208)])
+@pytest.mark.parametrize("mask", ["causal prefix", "causal cap", "causal bias", "causal cap bias prefix"])
+@pytest.mark.parametrize("form", ["four waves", "one wave", "split"])
+def test_docs_rows_taken_again_with_every_score(cuda, heads, kv_heads, hd, mask, form):
+    """Rows whose tile holds an infinity or NaN of v that they do not see, with prefixes, capped and biased scores; rows
+    that see no key among them."""
+    from mme import ops
+    g = gen(hd + len(mask))
+    few = form == "split"
+    qlens = [5, 2, 7] if few else [90, 41, 20] + [30] * (160 if form == "one wave" else 0)
+    klens = [1500, 900, 4] if few else [90, 60, 12] + [30] * (len(qlens) - 3)
+    q, k, v = make(g, sum(qlens), sum(klens), heads, kv_heads, hd, cuda)
+    off, koff = cuts(qlens).to(cuda), cuts(klens).to(cuda)
+    kw = scores(mask, heads, klens, cuda)
+    if "prefix" in kw:
+        kw["prefix"][1:3] = torch.tensor([klens[1] - 9, 0], dtype=torch.int32, device=cuda)
+    blind = np.zeros((sum(qlens), 1), bool)   # rows that do not see their document's bad key
+    for d, (m, n) in enumerate(zip(qlens, klens)):
+        at = n - 2
+        v[int(koff[d]) + at] = (float("inf"), float("nan"), -float("inf"))[d % 3]
+        pre = int(kw["prefix"][d]) if "prefix" in kw else 0
+        blind[int(off[d]):int(off[d]) + m, 0] = [max(i + n - m + 1, pre) <= at for i in range(m)]
+    got = ops.attention_docs(q, k, v, off, heads, kv_heads, key_offsets=koff, max_rows=max(qlens), **kw)
+    assert blind.any() and torch.isfinite(got[torch.from_numpy(blind[:, 0]).to(cuda)].float()).all()
+    seeing = torch.from_numpy(~blind[:, 0]).to(cuda)
+    assert not torch.isfinite(got[seeing].float()).any()
+    # check_docs' bound holds: the weights of a row taken again are not rounded
+    check_docs(got, q, k, v, off, heads, kv_heads, rows=blind[:, 0], key_offsets=koff, **kw)
+    assert (got[int(off[2]):int(off[2]) + qlens[2] - klens[2]] == 0).all() or qlens[2] <= klens[2]
