@@ -413,10 +413,12 @@ int mme_rope_axes(const void* x, long ldx, void* y, long ldy, int rows, int nhea
  * device and joined). q: bf16 [rows_q, ldq], head h at column h*hd; k, v: bf16 [rows_k, ld], key head h / (Hq/Hkv);
  * out: bf16 [rows_q, ldo]. hd: multiples of 8 up to 128, of 16 up to 256. 16-byte aligned pointers, leading dims
  * % 8 == 0, those of k and v under 2^24. fp32 scores, softmax and sums; the weights are rounded to bf16 for the matrix
- * instruction. out must not share an element with q, k or v
- * (refused; columns of one buffer are no overlap).
- * workspace >= mme_attention_docs_workspace_bytes(...); 0 (it may be null), unless max_rows * Hq / Hkv <= 256 and
- * rows_k * hd >= 40960 * n. */
+ * instruction. out must not share an element with q, k or v (refused; columns of one buffer are no overlap).
+ * Room between the keys of two documents (a cache that grows) is a document without query rows:
+ * q_offsets 0 1 1 2, k_offsets 0 900 1024 2000. The keys are split by rows_k / n to a document: pass the rows in use,
+ * not all that a buffer has.
+ * workspace >= mme_attention_docs_workspace_bytes(...); 0 (it may be null), unless min(max_rows, rows_q) * Hq / Hkv <= 256
+ * and rows_k * hd >= 40960 * n. */
 size_t mme_attention_docs_workspace_bytes(int n, int rows_q, int rows_k, int Hq, int Hkv, int hd, int max_rows);
 int mme_attention_docs(const void* q, long ldq, const void* k, long ldk, const void* v, long ldv, void* out, long ldo,
                        const int32_t* q_offsets, const int32_t* k_offsets, int n, int rows_q, int rows_k, int Hq,

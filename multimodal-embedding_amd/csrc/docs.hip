@@ -212,12 +212,13 @@ __device__ __forceinline__ void row_alone(const DocsArgs& a, const Doc& D, int g
     }
 }
 
-// Whole calls measured beside a matrix product's 1 400 TF/s and a copy's 5.2 TB/s, and what bounds them:
+// Whole calls measured beside a matrix product's 1 400 TF/s and a copy's 5.2 TB/s, and what bounds them (MFMA busy: of
+// the SIMD cycles of CUs that had waves; of all 256 CUs through the kernel it is 30 / 43 / 53 %):
 //   12 pages of 1 030 - 1 100 tokens, 8 heads to 1 of 256, prefix, capped: 142 - 165 us, 0.64 - 0.74 PF/s. 806
-//     workgroups over the 512 places that 256 registers leave are two rounds, the second part full; MFMA 43 % busy.
+//     workgroups over the 512 places that 256 registers leave are two rounds, the second part full; MFMA 38 % busy.
 //   14 images of 64 - 2 916 patches, 16 heads of 72: 118 - 126 us, 0.67 - 0.72 PF/s; 72 is padded to 80 and 96 columns, and
-//     the softmax's vector instructions share the issue with MFMA (50 % busy).
-//   3 texts, the longest 6 143, 32 heads to 8 of 128, causal: 296 - 322 us, 0.96 - 1.05 PF/s; MFMA 57 % busy.
+//     the softmax's vector instructions share the issue with MFMA (53 % busy).
+//   3 texts, the longest 6 143, 32 heads to 8 of 128, causal: 296 - 322 us, 0.96 - 1.05 PF/s; MFMA 59 % busy.
 //   256 captions of 5 - 77 tokens, 12 heads of 64, biased: 15 us; a wave's chain of a copy, a product, a softmax.
 //   One query against 1 030 keys: 14 us, two launches, latency; 64 against 256 - 4 096 keys, 16 heads of 72: 92 us, 4.4 TB/s;
 //     5 against 3 001 - 65 536 keys, 8 key heads of 128: 160 us, 4.8 TB/s.
@@ -409,7 +410,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
     auto score = [&](auto cut_c, f32x16(&sc)[KB], int t) __attribute__((always_inline)) {
         constexpr bool CUT = decltype(cut_c)::value;
         const int key0 = key_lo + t * KT;
-        if (MODE & 1) {  // cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)), log2(e) folded in
+        if (MODE & 1) {
+            // cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)), log2(e) folded in: the exponential and reciprocal
+            // units' errors and the difference are worth 3 steps of the cap (4e-4 at a cap of 1 000, 2e-5 at 50)
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -735,8 +738,10 @@ Plan make_plan(int n, int rows_q, int rows_k, int Hkv, int group, int hd, int ma
     p.per = p.NW * 32;
     p.row_blocks = 1;
     long nslots = flat / p.per + n;
-    // Few flat rows a document: its keys in parts, for nearly three rounds of the workgroups that fit the device by
-    // their LDS (documents of different lengths at just over two rounds 195 us, at 2.7 157: the last is half empty).
+    // Few flat rows a document: its keys in parts. The bound of 256 keeps the workspace small and is not a measured
+    // optimum: beyond it the keys stay whole, and few such documents leave most CUs idle (8 heads to 1 of 256 against
+    // 65 536 keys: 32 queries 95 us in parts, 33 queries 4.6 ms whole).
+    // As many parts as make nearly three rounds of the workgroups that fit the device by their LDS (documents of different lengths at just over two rounds 195 us, at 2.7 157: the last is half empty).
     // Two parts at least, and enough for a workgroup to read without: one query against 512 / 1 024 / 4 096 keys of 8
     // documents, 8 heads of 128, whole 14.9 / 23 / 81 us, in parts 14.7 / 17 / 43; 16 documents, 16 heads of 72, 1 024 /
     // 4 096 keys 21 / 85 and 25 / 71 (more workgroups need longer documents). Documents of 1 353 keys on average, 256

@@ -549,8 +549,9 @@ def attention_docs(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: t
 
     q: bf16 [rows, heads * hd]; k, v: bf16 [key rows, kv_heads * hd] (views of packed q | k | v rows will do); each
     key head serves heads / kv_heads query heads. offsets: int32 [n + 1], where each document's query rows begin;
-    key_offsets: the same for the keys (default: offsets). Query i of a document stands at key position
-    i + klen - qlen. causal: it sees keys up to its own position, and with prefix (int32 [n]) also the document's
+    key_offsets: the same for the keys (default: offsets; room between two documents' keys, as in a cache that grows, is a
+    document without query rows, and k and v best end with the rows in use). Query i of a document stands at key
+    position i + klen - qlen. causal: it sees keys up to its own position, and with prefix (int32 [n]) also the document's
     first prefix[d] keys. softcap (0 for none, or 1e-3 to 1e3): scores become softcap * tanh(score / softcap).
     slopes (fp32 [heads]): scores lose slopes[h] * distance. scale: positive (default: hd ** -0.5). A query that sees no
     key gets zeros; keys that it does not see add nothing, whatever they hold. max_rows: no document has more query rows than this; give it where rows are few and keys many (one
