@@ -741,7 +741,8 @@ Plan make_plan(int n, int rows_q, int rows_k, int Hkv, int group, int hd, int ma
     // Few flat rows a document: its keys in parts. The bound of 256 keeps the workspace small and is not a measured
     // optimum: beyond it the keys stay whole, and few such documents leave most CUs idle (8 heads to 1 of 256 against
     // 65 536 keys: 32 queries 95 us in parts, 33 queries 4.6 ms whole).
-    // As many parts as make nearly three rounds of the workgroups that fit the device by their LDS (documents of different lengths at just over two rounds 195 us, at 2.7 157: the last is half empty).
+    // As many parts as make nearly three rounds of the workgroups that fit the device by their LDS (documents of
+    // different lengths at just over two rounds 195 us, at 2.7 157: the last is half empty).
     // Two parts at least, and enough for a workgroup to read without: one query against 512 / 1 024 / 4 096 keys of 8
     // documents, 8 heads of 128, whole 14.9 / 23 / 81 us, in parts 14.7 / 17 / 43; 16 documents, 16 heads of 72, 1 024 /
     // 4 096 keys 21 / 85 and 25 / 71 (more workgroups need longer documents). Documents of 1 353 keys on average, 256
